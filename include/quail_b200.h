@@ -337,6 +337,126 @@ int qb_answer_score(const void* normed, int64_t n_rows, int64_t hidden_dim, cons
                     int n_ids, const int32_t* true_cols, int n_true, const int32_t* false_cols,
                     int n_false, float* score_out, void* stream);
 
+/*
+ * ---- generation: the 8-bit KV cache, attention of one new token, beams ----
+ *
+ * The reference scores rows by prefill alone; these continue a row from the
+ * KV that a prefill left in the arena. They replace nothing in it.
+ */
+
+/*
+ * Quantises K and V rows into an 8-bit paged cache as they are written:
+ * for i < n with dst[i] >= 0, row src[i] (i when src is NULL) of k and v goes
+ * to pool row dst[i]; a negative dst[i] writes nothing. Per row and head the
+ * scale is 2^(b - 127), the least power of two with max |x| <= 448 * scale
+ * (max |x| taken as 1e-10 at least), the codes are e4m3(x / scale) rounded to
+ * nearest even, and b is the scale byte (E8M0). A head that holds an infinity
+ * or a NaN gets b = 255 and NaN codes.
+ * k, v: bf16, row r's heads at k + r * k_ld, head_dim apart (a slice of a
+ * wider projection); k_ld, v_ld in elements, multiples of 8, at least
+ * n_kv * head_dim; src, dst: int64 [n]; k_codes, v_codes: fp8 [pool_rows,
+ * n_kv, head_dim]; k_scale, v_scale: u8 [pool_rows, n_kv]. head_dim 64 or
+ * 128; k, v and the codes 16-byte aligned. The dst that are not negative must
+ * differ. A row index out of range sets QB_STATUS_BAD_INDEX and is skipped.
+ */
+int qb_kv_quant_write(const void* k, const void* v, int64_t k_ld, int64_t v_ld,
+                      const int64_t* src, const int64_t* dst, int64_t n,
+                      int64_t src_rows, int n_kv, int head_dim, void* k_codes,
+                      void* v_codes, uint8_t* k_scale, uint8_t* v_scale,
+                      int64_t pool_rows, void* stream);
+
+/*
+ * Reads rows of an 8-bit cache back as bf16: row dst[i] (i when dst is NULL;
+ * a negative dst[i] writes nothing) of k and v becomes code * 2^(b - 127) of
+ * pool row src[i]. Exact, except that a magnitude that rounded up past
+ * bf16's largest becomes an infinity. Shapes and alignments as
+ * qb_kv_quant_write; k and v have out_rows rows. A src out of range sets
+ * QB_STATUS_BAD_INDEX and gives zeros.
+ */
+int qb_kv_quant_read(const void* k_codes, const void* v_codes,
+                     const uint8_t* k_scale, const uint8_t* v_scale,
+                     int64_t pool_rows, const int64_t* src, const int64_t* dst,
+                     int64_t n, int n_kv, int head_dim, void* k, void* v,
+                     int64_t k_ld, int64_t v_ld, int64_t out_rows, void* stream);
+
+/*
+ * Attention of one new token per row over its paged KV cache: row r's query
+ * head h attends to keys 0 .. used[r] - 1 of KV head h / (n_q / n_kv), key i
+ * at pool row table[r][i / page_tokens] * page_tokens + i % page_tokens
+ * (the new token's own key and value already written there):
+ * out = softmax(q . k * softmax_scale) v, lse = ln sum e^(q . k *
+ * softmax_scale). A row with used[r] = 0, or whose every product is -inf, gets
+ * zeros and -inf. An infinity among V gives NaN.
+ * q: bf16, row r's heads at q + r * q_ld (q_ld a multiple of 8);
+ * k_scale NULL: bf16 pools [n_pages * page_tokens, n_kv, head_dim]; else the
+ * 8-bit cache of qb_kv_quant_write; table: int32 [rows, table_width], rows
+ * table_ld apart; used: int32 [rows]. Any of the outputs may be NULL but not
+ * out and q_out both: out: bf16, rows out_ld apart (a multiple of 4);
+ * q_out: fp8 [rows, n_q * 128] with scale_out f32 [n_q, scale_ld], the bf16
+ * output quantised per head as qb_tree_attention's (head_dim 128 only);
+ * lse_out: f32 [rows, n_q]. n_q a multiple of n_kv; head_dim 64 or 128;
+ * page_tokens a power of two from 8 to 1024; rows <= 65,535; q and the pools
+ * 16-byte aligned. A page or a used[r] out of range sets
+ * QB_STATUS_BAD_INDEX; such keys are left out.
+ */
+int qb_decode_attention(const void* q, int64_t q_ld, int64_t rows, int n_q,
+                        int n_kv, int head_dim, const void* k_pool,
+                        const void* v_pool, const uint8_t* k_scale,
+                        const uint8_t* v_scale, int64_t n_pages, int page_tokens,
+                        const int32_t* table, int64_t table_width,
+                        int64_t table_ld, const int32_t* used, float softmax_scale,
+                        void* out, int64_t out_ld, void* q_out, float* scale_out,
+                        int64_t scale_ld, int ue8m0, float* lse_out, void* stream);
+
+/* Bytes of workspace that qb_beam_select needs for these sizes. */
+int qb_beam_select_workspace(int64_t groups, int beams, int64_t vocab, int n_out,
+                             int64_t* bytes);
+
+/*
+ * Beam search's choice over beams and vocabulary. Beam b of a group scores
+ * its continuation by token v with scores[b] + (x_bv - lse_b), lse_b = ln
+ * sum_v e^(x_bv). Each beam offers its n_out largest logits (equal ones: lowest
+ * token first); the group's n_out best offers are returned in order (equal
+ * scores: lowest beam first, then the beam's order). A finished beam offers
+ * itself alone, with its score unchanged and the token `pad`; its logits are
+ * not read. Logits of -inf are tokens that are not allowed. A beam whose
+ * logits hold a NaN or +inf, or nothing but -inf, offers at -inf.
+ * logits: f32 (or bf16 when logits_bf16) [groups * beams, vocab], rows
+ * logits_ld apart; scores: f32 [groups, beams]; finished: u8 [groups, beams] or
+ * NULL; scores_out: f32, parent_out: int32 (beam within the group), token_out:
+ * int64, each [groups, n_out]. 1 to 32 beams and n_out, vocab >= n_out.
+ */
+int qb_beam_select(const void* logits, int logits_bf16, int64_t logits_ld,
+                   int64_t groups, int beams, int64_t vocab, const float* scores,
+                   const uint8_t* finished, int64_t pad, int n_out, void* workspace,
+                   int64_t workspace_bytes, float* scores_out, int32_t* parent_out,
+                   int64_t* token_out, void* stream);
+
+/*
+ * Reorders the beams' paged KV to follow a choice. Every beam of group g
+ * holds used[g] tokens; the table entries before used[g] / page_tokens are
+ * full pages that beams may share, the others (the started page and any
+ * reserved ones) are the beam's own. Child j of parent p = parents[g][j]
+ * gets p's full pages and
+ *   - p's own pages, when no earlier child has p as its parent, or
+ *   - the own pages of a beam without children (the e-th such child those of
+ *     the e-th such beam), into which p's started tokens are copied.
+ * So no copied page is written and every page keeps one owner.
+ * parents: int32 [groups, beams]; used: int32 [groups]; table_in, table_out:
+ * int32 [groups * beams, table_width], not the same memory; pool: n_slabs
+ * slabs (a layer's K or V) of n_pages * page_tokens rows of row_bytes (a
+ * multiple of 16), contiguous; pool2: a second pool over the same rows (an
+ * 8-bit cache's scales) or NULL; next_row: int64 [groups * beams] or NULL, the
+ * pool row of each child's next token (-1 when its table is full). 1 to 32
+ * beams; groups * beams <= 65,535. A parent or page out of range sets
+ * QB_STATUS_BAD_INDEX.
+ */
+int qb_beam_reorder(const int32_t* parents, const int32_t* used, int64_t groups,
+                    int beams, const int32_t* table_in, int64_t table_width,
+                    int page_tokens, int64_t n_pages, void* pool, int64_t n_slabs,
+                    int64_t row_bytes, void* pool2, int64_t row_bytes2,
+                    int32_t* table_out, int64_t* next_row, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

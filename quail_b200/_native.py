@@ -53,6 +53,17 @@ SIGNATURES = {
     "qb_final_norm": [_P, _P, _I64, _I64, _P, _I64, _P, _F32, _P, _P],
     "qb_answer_margin": [_P, _I64, _I64, _P, _I32, _P, _I32, _P, _I32, _P, _P, _P],
     "qb_answer_score": [_P, _I64, _I64, _P, _I32, _P, _I32, _P, _I32, _P, _P],
+    "qb_kv_quant_write": [_P, _P, _I64, _I64, _P, _P, _I64, _I64, _I32, _I32, _P, _P, _P, _P,
+                          _I64, _P],
+    "qb_kv_quant_read": [_P, _P, _P, _P, _I64, _P, _P, _I64, _I32, _I32, _P, _P, _I64, _I64,
+                         _I64, _P],
+    "qb_decode_attention": [_P, _I64, _I64, _I32, _I32, _I32, _P, _P, _P, _P, _I64, _I32, _P,
+                            _I64, _I64, _P, _F32, _P, _I64, _P, _P, _I64, _I32, _P, _P],
+    "qb_beam_select_workspace": [_I64, _I32, _I64, _I32, _P],
+    "qb_beam_select": [_P, _I32, _I64, _I64, _I32, _I64, _P, _P, _I64, _I32, _P, _I64, _P, _P,
+                       _P, _P],
+    "qb_beam_reorder": [_P, _P, _I64, _I32, _P, _I64, _I32, _I64, _P, _I64, _I64, _P, _I64, _P,
+                        _P, _P],
 }
 
 _lib = None
@@ -98,7 +109,7 @@ def check(status: int, what: str) -> None:
 # entry points that launch a kernel; LAUNCHES counts them per process
 LAUNCHING = frozenset(n for n in SIGNATURES if n not in (
     "qb_version", "qb_last_error", "qb_kernel_status", "qb_set_wait_limit",
-    "qb_tree_attention_tiles"))
+    "qb_tree_attention_tiles", "qb_beam_select_workspace"))
 LAUNCHES = {"count": 0}
 
 

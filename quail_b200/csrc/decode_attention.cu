@@ -1,0 +1,561 @@
+// Attention of one new token per row over its paged KV cache (bf16 pools, or
+// the 8-bit pools of kv_quant.cu).
+//
+// For row r and query head h, with j = h / (n_q / n_kv) its KV head and key i
+// (i < used[r]) at pool row table[r][i / P] * P + i % P:
+//   x_i = q . k_i * softmax_scale * log2(e),  m = max x_i,
+//   out = sum 2^(x_i - m) v_i / sum 2^(x_i - m),
+//   lse = ln 2 * m + ln sum 2^(x_i - m).
+// An 8-bit key is code * 2^kb and value code * 2^vb (one exponent byte per
+// row and head): 2^kb multiplies x_i, and vb is added to the exponent of the
+// weight that meets the value's codes.
+//
+// HBM-bound: every K and V element is read once and meets n_q / n_kv query
+// heads (4 to 8 here), 4 to 16 flop a byte. The few heads of one KV head are
+// the N = 8 columns of mma.sync m16n8k16: S^T = K Q^T with 16 keys as rows,
+// then O^T = V^T P^T with 16 of the head's dimensions as rows. tcgen05's
+// smallest tile has 64 rows and wants its operands in shared memory by way of
+// descriptors; here a lane's 16-byte global loads are the operand fragments
+// themselves (the inner dimension's order is free, so each lane takes the
+// columns that it loaded), and nothing is staged.
+#include <cuda_fp16.h>
+
+#include "common.cuh"
+
+namespace {
+
+using namespace qb;
+
+constexpr int WARPS = 8;      // of one block; they take a head's key steps in turn
+constexpr int HEADS = 8;      // query heads of a block: the MMA's N
+constexpr float LN2 = 0.693147180559945309f;
+constexpr float LOG2E = 1.44269504088896341f;
+
+struct Params {
+    const bf16* q;
+    int64_t q_ld;
+    int n_q, n_kv, group;             // group = n_q / n_kv
+    int tiles;                        // ceil(group / HEADS) blocks share a KV head
+    const void* k;
+    const void* v;
+    const uint8_t* k_scale;
+    const uint8_t* v_scale;
+    int64_t n_pages;
+    int page_shift;                   // log2 of the page's tokens
+    const int32_t* table;
+    int64_t table_width, table_ld;
+    const int32_t* used;
+    float scale_log2;                 // softmax_scale * log2(e)
+    bf16* out;
+    int64_t out_ld;
+    uint8_t* q_out;
+    float* scale_out;
+    int64_t scale_ld;
+    bool ue8m0;
+    float* lse;
+    uint32_t* status;
+};
+
+// 16 (or 8) bytes of the pools: read once, so not kept in L1
+__device__ __forceinline__ uint4 load16(const void* p) {
+    uint4 r;
+    asm volatile("ld.global.nc.L1::no_allocate.v4.u32 {%0, %1, %2, %3}, [%4];"
+                 : "=r"(r.x), "=r"(r.y), "=r"(r.z), "=r"(r.w) : "l"(p));
+    return r;
+}
+__device__ __forceinline__ uint2 load8(const void* p) {
+    uint2 r;
+    asm volatile("ld.global.nc.L1::no_allocate.v2.u32 {%0, %1}, [%2];"
+                 : "=r"(r.x), "=r"(r.y) : "l"(p));
+    return r;
+}
+
+__device__ __forceinline__ float exp2_approx(float x) {
+    float r;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
+    return r;
+}
+
+// e4m3 pair (low half of c) -> f16 pair, exactly
+__device__ __forceinline__ uint32_t e4m3x2_f16x2(uint32_t c) {
+    uint32_t r;
+    asm("cvt.rn.f16x2.e4m3x2 %0, %1;" : "=r"(r) : "h"((uint16_t)c));
+    return r;
+}
+
+template <bool F16>
+__device__ __forceinline__ void mma16816(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2,
+                                         uint32_t a3, uint32_t b0, uint32_t b1) {
+    if (F16)
+        asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, "
+            "{%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
+            : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+            : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+    else
+        asm("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0, %1, %2, %3}, "
+            "{%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
+            : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+            : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+
+// the 8x8 transpose of a warp's 16-bit matrix (lane: row lane / 4, columns
+// 2 (lane % 4) and the next)
+__device__ __forceinline__ uint32_t transpose8(uint32_t a) {
+    uint32_t r;
+    asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(r) : "r"(a));
+    return r;
+}
+
+__device__ __forceinline__ uint32_t half2_bits(float a, float b) {
+    const __half2 h = __floats2half2_rn(a, b);
+    return *reinterpret_cast<const uint32_t*>(&h);
+}
+
+// 2^(b - 127) of an exponent byte; 255 is NaN
+__device__ __forceinline__ float e8m0_float(uint32_t b) {
+    if (b == 255u) return __uint_as_float(0x7FFFFFFFu);
+    return __uint_as_float(b ? b << 23 : 0x00400000u);
+}
+
+// One block: one row, one KV head, up to 8 of its query heads. Warp w takes
+// the key steps w, w + 8, ...; the warps' partial results meet in shared
+// memory at the end.
+//
+// Lanes: g = lane / 4, t = lane % 4, as the MMA fragments number them.
+template <int D, bool FP8>
+__global__ void __launch_bounds__(WARPS * 32)
+decode_attention_kernel(const Params p) {
+    constexpr int STEP = 16;                     // keys of a warp's step
+    constexpr int ELEM = FP8 ? 1 : 2;
+    constexpr int KC = D * ELEM / 64;            // 16-byte chunks of a K row a lane
+    constexpr int VC = FP8 ? 1 : D / 64;         // chunks of a V row a lane
+    constexpr int MT = D / 16;                   // 16-row tiles of O^T
+    __shared__ float s_o[WARPS][HEADS][D + 4];
+    __shared__ float s_m[WARPS][HEADS], s_l[WARPS][HEADS], s_mv[WARPS][HEADS];
+
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    const int g = lane >> 2, t = lane & 3;
+    const int row = blockIdx.y;
+    const int kvh = blockIdx.x / p.tiles, tile = blockIdx.x % p.tiles;
+    const int head0 = kvh * p.group + tile * HEADS;              // first query head
+    const int heads = min(HEADS, p.group - tile * HEADS);
+    const int page = 1 << p.page_shift;
+    const int32_t* table = p.table + row * p.table_ld;
+
+    int used = p.used[row];
+    if (used < 0 || used > (p.table_width << p.page_shift)) {
+        if (threadIdx.x == 0) atomicOr(p.status, STATUS_BAD_INDEX);
+        used = used < 0 ? 0 : (int)(p.table_width << p.page_shift);
+    }
+
+    // Q as the B fragments of S^T: this lane's columns of head g
+    uint32_t qf[D / 8];
+    float x_scale[2] = {p.scale_log2, p.scale_log2};   // of heads 2t and 2t + 1
+    {
+        const bf16* q = p.q + row * p.q_ld + (int64_t)(head0 + g) * D;
+        constexpr int QC = D / 32;   // 16-byte chunks of Q a lane
+        uint4 raw[QC];
+#pragma unroll
+        for (int c = 0; c < QC; ++c) {
+            // bf16: the K lane's chunks t + 4 c; 8 bit: K chunk t + 4 j holds
+            // 16 columns, two chunks of Q
+            const int at = FP8 ? 2 * (t + 4 * (c >> 1)) + (c & 1) : t + 4 * c;
+            raw[c] = g < heads ? *reinterpret_cast<const uint4*>(q + at * 8)
+                               : make_uint4(0, 0, 0, 0);
+        }
+        if (!FP8) {
+#pragma unroll
+            for (int c = 0; c < QC; ++c) {
+                qf[4 * c] = raw[c].x; qf[4 * c + 1] = raw[c].y;
+                qf[4 * c + 2] = raw[c].z; qf[4 * c + 3] = raw[c].w;
+            }
+        } else {
+            // f16 operands: q 2^-e with its largest element in [2^14, 2^15),
+            // exact down to 2^-28 of that element
+            uint32_t top = 0;
+            float x[QC][8];
+#pragma unroll
+            for (int c = 0; c < QC; ++c) {
+                bf16x8_to_float(raw[c], x[c]);
+#pragma unroll
+                for (int i = 0; i < 8; ++i)
+                    top = max(top, __float_as_uint(x[c][i]) & 0x7FFFFFFFu);
+            }
+            top = max(top, __shfl_xor_sync(0xffffffffu, top, 1));
+            top = max(top, __shfl_xor_sync(0xffffffffu, top, 2));
+            int e = (int)(top >> 23) - 127 - 14;
+            if (top >= 0x7F800000u || top == 0) e = 0;
+            e = max(e, -100);
+            const float down = __uint_as_float((uint32_t)(127 - e) << 23);
+            const float up = __uint_as_float((uint32_t)(127 + e) << 23);
+#pragma unroll
+            for (int c = 0; c < QC; ++c)
+#pragma unroll
+                for (int i = 0; i < 4; ++i)
+                    qf[4 * c + i] = half2_bits(x[c][2 * i] * down, x[c][2 * i + 1] * down);
+            x_scale[0] *= __shfl_sync(0xffffffffu, up, 8 * t);
+            x_scale[1] *= __shfl_sync(0xffffffffu, up, 8 * t + 4);
+        }
+    }
+
+    // Running state of heads 2t and 2t + 1. ref is the exponent that the
+    // weights are taken against: the largest x when it was last raised (0
+    // before any), raised only when an x passes it by more than SLACK, so that
+    // most steps need one vote and no reduction.
+    constexpr float SLACK = FP8 ? 2.0f : 8.0f;
+    // 8 bit: weights of the values are taken against the largest x + vb and
+    // shifted up, so that f16 holds them to 2^-27 of the largest before they
+    // become subnormal (2^(13 + 2) at most)
+    constexpr float LIFT = 13.0f;
+    const float NEG_INF = __uint_as_float(0xFF800000u);
+    float top[2] = {NEG_INF, NEG_INF}, ref[2] = {0.0f, 0.0f}, sum[2] = {0.0f, 0.0f};
+    float top_v[2] = {NEG_INF, NEG_INF}, ref_v[2] = {0.0f, 0.0f};
+    float o[MT][4];
+#pragma unroll
+    for (int i = 0; i < MT; ++i)
+#pragma unroll
+        for (int j = 0; j < 4; ++j) o[i][j] = 0.0f;
+
+    const int64_t row_bytes = (int64_t)p.n_kv * D * ELEM;
+    const char* k_base = (const char*)p.k + (int64_t)kvh * D * ELEM;
+    const char* v_base = (const char*)p.v + (int64_t)kvh * D * ELEM;
+
+    for (int key0 = warp * STEP; key0 < used; key0 += WARPS * STEP) {
+        // a page holds a multiple of 8 tokens, so each half step is in one page
+        int64_t half_row[2];
+        bool half_ok[2];
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+            const int key = key0 + 8 * h;
+            const int id = key < used ? table[key >> p.page_shift] : 0;
+            half_ok[h] = key < used && id >= 0 && id < p.n_pages;
+            if (key < used && !half_ok[h] && lane == 0) atomicOr(p.status, STATUS_BAD_INDEX);
+            half_row[h] = ((int64_t)(half_ok[h] ? id : 0) << p.page_shift) + (key & (page - 1));
+        }
+        // ---- K: rows g and g + 8 of the step
+        uint4 kr[2][KC];
+        float kx[2] = {1.0f, 1.0f};
+        bool k_ok[2];
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+            k_ok[h] = half_ok[h] && key0 + 8 * h + g < used;
+            const int64_t at = half_row[h] + g;
+#pragma unroll
+            for (int c = 0; c < KC; ++c)
+                kr[h][c] = k_ok[h] ? load16(k_base + at * row_bytes + (t + 4 * c) * 16)
+                                   : make_uint4(0, 0, 0, 0);
+            if (FP8 && k_ok[h]) kx[h] = e8m0_float(p.k_scale[at * p.n_kv + kvh]);
+        }
+        // ---- V: rows 2t, 2t + 1 of each half; codes of keys past the end
+        // are zeros, for 0 * NaN is NaN
+        uint4 vr[4][VC];
+        float vb[2] = {0.0f, 0.0f};   // exponents of keys g and g + 8
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+            const int h = r >> 1, off = 2 * t + (r & 1);
+            const bool ok = half_ok[h] && key0 + 8 * h + off < used;
+            const int64_t at = half_row[h] + off;
+#pragma unroll
+            for (int c = 0; c < VC; ++c) {
+                vr[r][c] = make_uint4(0, 0, 0, 0);
+                if (FP8 && D == 64) {
+                    if (ok) {
+                        const uint2 w = load8(v_base + at * row_bytes + g * 8);
+                        vr[r][c].x = w.x;
+                        vr[r][c].y = w.y;
+                    }
+                } else if (ok) {
+                    vr[r][c] = load16(v_base + at * row_bytes + (g + 8 * c) * 16);
+                }
+            }
+        }
+        if (FP8) {
+#pragma unroll
+            for (int h = 0; h < 2; ++h)
+                if (k_ok[h]) {
+                    const uint32_t b = p.v_scale[(half_row[h] + g) * p.n_kv + kvh];
+                    vb[h] = b == 255u ? __uint_as_float(0x7FFFFFFFu) : (float)((int)b - 127);
+                }
+        }
+
+        // ---- S^T: keys g and g + 8, heads 2t and 2t + 1
+        float s[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+        for (int c = 0; c < KC; ++c) {
+            const uint32_t w0[4] = {kr[0][c].x, kr[0][c].y, kr[0][c].z, kr[0][c].w};
+            const uint32_t w1[4] = {kr[1][c].x, kr[1][c].y, kr[1][c].z, kr[1][c].w};
+            if (FP8) {
+#pragma unroll
+                for (int w = 0; w < 4; ++w)
+                    mma16816<true>(s, e4m3x2_f16x2(w0[w]), e4m3x2_f16x2(w1[w]),
+                                   e4m3x2_f16x2(w0[w] >> 16), e4m3x2_f16x2(w1[w] >> 16),
+                                   qf[8 * c + 2 * w], qf[8 * c + 2 * w + 1]);
+            } else {
+#pragma unroll
+                for (int w = 0; w < 2; ++w)
+                    mma16816<false>(s, w0[2 * w], w1[2 * w], w0[2 * w + 1], w1[2 * w + 1],
+                                    qf[4 * c + 2 * w], qf[4 * c + 2 * w + 1]);
+            }
+        }
+        float x[4], y[4];   // index 2 * half + head; y: the exponent with the value's scale
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            x[i] = s[i] * x_scale[i & 1];
+            if (FP8) x[i] *= kx[i >> 1];
+            if (!k_ok[i >> 1]) x[i] = NEG_INF;
+            y[i] = FP8 ? x[i] + vb[i >> 1] : x[i];
+        }
+        bool raise = false;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            raise |= x[i] > top[i & 1] + SLACK;
+            if (FP8) raise |= y[i] > top_v[i & 1] + SLACK;
+        }
+        if (__any_sync(0xffffffffu, raise)) {
+#pragma unroll
+            for (int n = 0; n < 2; ++n) {
+                float a = fmaxf(x[n], x[2 + n]), b = fmaxf(y[n], y[2 + n]);
+#pragma unroll
+                for (int off = 4; off < 32; off <<= 1) {
+                    a = fmaxf(a, __shfl_xor_sync(0xffffffffu, a, off));
+                    if (FP8) b = fmaxf(b, __shfl_xor_sync(0xffffffffu, b, off));
+                }
+                a = fmaxf(a, top[n]);
+                const float old = ref[n];
+                float down = 0.0f;
+                if (a > NEG_INF) {
+                    ref[n] = a;
+                    if (top[n] > NEG_INF) down = exp2_approx(old - a);
+                }
+                top[n] = a;
+                sum[n] *= down;
+                if (FP8) {
+                    b = fmaxf(b, top_v[n]);
+                    const float old_v = ref_v[n];
+                    down = 0.0f;
+                    if (b > NEG_INF) {
+                        ref_v[n] = b;
+                        if (top_v[n] > NEG_INF) down = exp2_approx(old_v - b);
+                    }
+                    top_v[n] = b;
+                }
+#pragma unroll
+                for (int i = 0; i < MT; ++i) {
+                    o[i][n] *= down;
+                    o[i][2 + n] *= down;
+                }
+            }
+        }
+        float w[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const float e = exp2_approx(x[i] - ref[i & 1]);
+            sum[i & 1] += e;
+            w[i] = FP8 ? exp2_approx(y[i] - ref_v[i & 1] + LIFT) : e;
+        }
+        // ---- O^T += V^T P^T: the weights as B fragments, by a transpose.
+        // bf16 keeps 8 bits of a weight, so what it drops goes through a second
+        // product; f16 keeps 11 and needs none.
+        uint32_t hi[2], lo[2];
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+            if (FP8) {
+                hi[h] = transpose8(half2_bits(w[2 * h], w[2 * h + 1]));
+            } else {
+                const uint32_t b = bf16x2_bits(w[2 * h], w[2 * h + 1]);
+                const float2 f = bf16x2_float2(b);
+                hi[h] = transpose8(b);
+                lo[h] = transpose8(bf16x2_bits(w[2 * h] - f.x, w[2 * h + 1] - f.y));
+            }
+        }
+#pragma unroll
+        for (int c = 0; c < VC; ++c) {
+            const uint32_t v0[4] = {vr[0][c].x, vr[0][c].y, vr[0][c].z, vr[0][c].w};
+            const uint32_t v1[4] = {vr[1][c].x, vr[1][c].y, vr[1][c].z, vr[1][c].w};
+            const uint32_t v2[4] = {vr[2][c].x, vr[2][c].y, vr[2][c].z, vr[2][c].w};
+            const uint32_t v3[4] = {vr[3][c].x, vr[3][c].y, vr[3][c].z, vr[3][c].w};
+#pragma unroll
+            for (int i = 0; i < (FP8 && D == 64 ? 2 : 4); ++i) {
+                if (FP8) {
+                    // four columns of keys 2t, 2t + 1 (a) and 2t + 8, 2t + 9 (b)
+                    const uint32_t a01 = __byte_perm(v0[i], v1[i], 0x5140);
+                    const uint32_t a23 = __byte_perm(v0[i], v1[i], 0x7362);
+                    const uint32_t b01 = __byte_perm(v2[i], v3[i], 0x5140);
+                    const uint32_t b23 = __byte_perm(v2[i], v3[i], 0x7362);
+                    mma16816<true>(o[2 * i], e4m3x2_f16x2(a01), e4m3x2_f16x2(a01 >> 16),
+                                   e4m3x2_f16x2(b01), e4m3x2_f16x2(b01 >> 16), hi[0], hi[1]);
+                    mma16816<true>(o[2 * i + 1], e4m3x2_f16x2(a23), e4m3x2_f16x2(a23 >> 16),
+                                   e4m3x2_f16x2(b23), e4m3x2_f16x2(b23 >> 16), hi[0], hi[1]);
+                } else {
+                    const uint32_t a0 = __byte_perm(v0[i], v1[i], 0x5410);
+                    const uint32_t a1 = __byte_perm(v0[i], v1[i], 0x7632);
+                    const uint32_t a2 = __byte_perm(v2[i], v3[i], 0x5410);
+                    const uint32_t a3 = __byte_perm(v2[i], v3[i], 0x7632);
+                    mma16816<false>(o[4 * c + i], a0, a1, a2, a3, hi[0], hi[1]);
+                    mma16816<false>(o[4 * c + i], a0, a1, a2, a3, lo[0], lo[1]);
+                }
+            }
+        }
+    }
+
+    // ---- the warp's sums, and its state to shared memory
+#pragma unroll
+    for (int n = 0; n < 2; ++n) {
+#pragma unroll
+        for (int off = 4; off < 32; off <<= 1)
+            sum[n] += __shfl_xor_sync(0xffffffffu, sum[n], off);
+        if (g == 0) {
+            s_m[warp][2 * t + n] = top[n] > NEG_INF || sum[n] != 0.0f ? ref[n] : NEG_INF;
+            s_l[warp][2 * t + n] = sum[n];
+            // (a finite x whose value exponent is NaN leaves top_v behind)
+            s_mv[warp][2 * t + n] =
+                top_v[n] > NEG_INF || top[n] > NEG_INF ? ref_v[n] : NEG_INF;
+        }
+#pragma unroll
+        for (int i = 0; i < MT; ++i)
+#pragma unroll
+            for (int e = 0; e < 2; ++e) {
+                // column of tile i, row g (e = 0) or g + 8 (e = 1)
+                const int d = FP8 ? (D / 8) * g + 2 * i + e
+                                  : 8 * (g + 8 * (i >> 2)) + 2 * (i & 3) + e;
+                s_o[warp][2 * t + n][d] = o[i][2 * e + n];
+            }
+    }
+    __syncthreads();
+
+    // ---- join: four columns of one head a thread
+    constexpr int QUADS = D / 4;
+    const int head = threadIdx.x / QUADS, d4 = (threadIdx.x % QUADS) * 4;
+    if (head >= HEADS) return;   // D = 64: half of the threads
+    float m = NEG_INF, mv = NEG_INF;
+#pragma unroll
+    for (int i = 0; i < WARPS; ++i) {
+        m = fmaxf(m, s_m[i][head]);
+        mv = fmaxf(mv, s_mv[i][head]);
+    }
+    float l = 0.0f, acc[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+    for (int i = 0; i < WARPS; ++i) {
+        const float mi = s_m[i][head];
+        if (mi > NEG_INF || s_l[i][head] != 0.0f) l += s_l[i][head] * exp2f(mi - m);
+        const float mvi = FP8 ? s_mv[i][head] : mi;
+        if (mvi == NEG_INF) continue;
+        const float f = exp2f(mvi - (FP8 ? mv : m));
+        const float4 part = *reinterpret_cast<const float4*>(&s_o[i][head][d4]);
+        acc[0] += f * part.x;
+        acc[1] += f * part.y;
+        acc[2] += f * part.z;
+        acc[3] += f * part.w;
+    }
+    float r[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+    if (l != 0.0f) {   // a NaN stays one
+        const float f = FP8 && mv > NEG_INF ? exp2f(mv - m - LIFT) : 1.0f;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) r[i] = acc[i] / l * f;
+    }
+    if (head < heads) {
+        const int64_t h = head0 + head;
+        if (p.lse && d4 == 0) p.lse[row * (int64_t)p.n_q + h] = l != 0.0f ? m * LN2 + logf(l) : NEG_INF;
+        if (p.out) {
+            uint2 b;
+            b.x = bf16x2_bits(r[0], r[1]);
+            b.y = bf16x2_bits(r[2], r[3]);
+            *reinterpret_cast<uint2*>(p.out + row * p.out_ld + h * D + d4) = b;
+        }
+    }
+    if (D == 128 && p.q_out) {
+        // o_proj's input: bf16 first, then the head's 128 columns as one
+        // quantisation group, as the prefill attention does; a warp holds a head
+        float b[4], amax = 0.0f;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            b[i] = bf16_round(r[i]);
+            amax = fmaxf(amax, fabsf(b[i]));
+        }
+        amax = warp_max(amax);
+        const float scale = p.ue8m0 ? ue8m0_scale(amax) : group_scale(amax);
+        const GroupDivider div(scale);
+        if (head < heads) {
+            const int64_t h = head0 + head;
+            const uint32_t lo = fp8x2(div.quant(b[0]), div.quant(b[1]));
+            const uint32_t hi = fp8x2(div.quant(b[2]), div.quant(b[3]));
+            *reinterpret_cast<uint32_t*>(p.q_out + row * (int64_t)p.n_q * D + h * D + d4) =
+                lo | (hi << 16);
+            if (d4 == 0) p.scale_out[h * p.scale_ld + row] = scale;
+        }
+    }
+}
+
+}  // namespace
+
+extern "C" int qb_decode_attention(const void* q, int64_t q_ld, int64_t rows, int n_q, int n_kv,
+                                   int head_dim, const void* k_pool, const void* v_pool,
+                                   const uint8_t* k_scale, const uint8_t* v_scale,
+                                   int64_t n_pages, int page_tokens, const int32_t* table,
+                                   int64_t table_width, int64_t table_ld, const int32_t* used,
+                                   float softmax_scale, void* out, int64_t out_ld, void* q_out,
+                                   float* scale_out, int64_t scale_ld, int ue8m0, float* lse_out,
+                                   void* stream) {
+    const char* who = "qb_decode_attention";
+    if (head_dim != 64 && head_dim != 128)
+        return invalid("qb_decode_attention: head_dim must be 64 or 128");
+    if (n_q <= 0 || n_kv <= 0 || n_q % n_kv)
+        return invalid("qb_decode_attention: n_q must be a positive multiple of n_kv");
+    if (rows < 0 || rows > 65535) return invalid("qb_decode_attention: 0 to 65,535 rows");
+    if (page_tokens < 8 || page_tokens > 1024 || (page_tokens & (page_tokens - 1)))
+        return invalid("qb_decode_attention: page_tokens must be a power of two from 8 to 1024");
+    const int64_t width = (int64_t)n_q * head_dim;
+    if (q_ld < width || q_ld % 8 || !aligned(q, 16))
+        return invalid("qb_decode_attention: q needs 16-byte alignment and q_ld a multiple of 8 "
+                       "that covers the heads");
+    if (!out && !q_out) return invalid("qb_decode_attention: no output");
+    if (out && (out_ld < width || out_ld % 4 || !aligned(out, 8)))
+        return invalid("qb_decode_attention: out needs 8-byte alignment and out_ld a multiple "
+                       "of 4 that covers the heads");
+    if (q_out && (head_dim != 128 || !scale_out || scale_ld < rows || !aligned(q_out, 4)))
+        return invalid("qb_decode_attention: the fp8 output needs head_dim 128, scale_out and "
+                       "scale_ld >= rows");
+    if (rows == 0) return QB_OK;
+    if (!q || !k_pool || !v_pool || !table || !used)
+        return invalid("qb_decode_attention: NULL tensor");
+    if ((k_scale == nullptr) != (v_scale == nullptr))
+        return invalid("qb_decode_attention: k_scale and v_scale go together");
+    if (!aligned(k_pool, 16) || !aligned(v_pool, 16))
+        return invalid("qb_decode_attention: the pools must be 16-byte aligned");
+    if (n_pages <= 0 || table_width <= 0 || table_ld < table_width ||
+        table_width > 0x7fffffffLL / page_tokens)
+        return invalid("qb_decode_attention: bad table width or page count");
+    Params p;
+    p.q = (const bf16*)q;
+    p.q_ld = q_ld;
+    p.n_q = n_q;
+    p.n_kv = n_kv;
+    p.group = n_q / n_kv;
+    p.tiles = (p.group + HEADS - 1) / HEADS;
+    p.k = k_pool;
+    p.v = v_pool;
+    p.k_scale = k_scale;
+    p.v_scale = v_scale;
+    p.n_pages = n_pages;
+    p.page_shift = __builtin_ctz((unsigned)page_tokens);
+    p.table = table;
+    p.table_width = table_width;
+    p.table_ld = table_ld;
+    p.used = used;
+    p.scale_log2 = softmax_scale * LOG2E;
+    p.out = (bf16*)out;
+    p.out_ld = out_ld;
+    p.q_out = (uint8_t*)q_out;
+    p.scale_out = scale_out;
+    p.scale_ld = scale_ld;
+    p.ue8m0 = ue8m0 != 0;
+    p.lse = lse_out;
+    p.status = device_status_ptr();
+    if (!p.status) return launch_status("qb_decode_attention: status word");
+    const dim3 grid((unsigned)(n_kv * p.tiles), (unsigned)rows);
+    auto* kernel = head_dim == 128 ? (k_scale ? decode_attention_kernel<128, true>
+                                              : decode_attention_kernel<128, false>)
+                                   : (k_scale ? decode_attention_kernel<64, true>
+                                              : decode_attention_kernel<64, false>);
+    kernel<<<grid, WARPS * 32, 0, (cudaStream_t)stream>>>(p);
+    return launch_status(who);
+}
