@@ -379,6 +379,10 @@ int qb_kv_quant_read(const void* k_codes, const void* v_codes,
                      int64_t n, int n_kv, int head_dim, void* k, void* v,
                      int64_t k_ld, int64_t v_ld, int64_t out_rows, void* stream);
 
+/* Bytes of workspace that qb_decode_attention needs on the current device,
+ * whatever the sizes. */
+int qb_decode_attention_workspace(int64_t* bytes);
+
 /*
  * Attention of one new token per row over its paged KV cache: row r's query
  * head h attends to keys 0 .. used[r] - 1 of KV head h / (n_q / n_kv), key i
@@ -398,6 +402,9 @@ int qb_kv_quant_read(const void* k_codes, const void* v_codes,
  * page_tokens a power of two from 8 to 1024; rows <= 65,535; q and the pools
  * 16-byte aligned. A page or a used[r] out of range sets
  * QB_STATUS_BAD_INDEX; such keys are left out.
+ * workspace: qb_decode_attention_workspace bytes, zero before its first call
+ * (each call leaves its counters zero); calls that may run at the same time
+ * need one each. The result does not depend on how blocks were scheduled.
  */
 int qb_decode_attention(const void* q, int64_t q_ld, int64_t rows, int n_q,
                         int n_kv, int head_dim, const void* k_pool,
@@ -405,7 +412,8 @@ int qb_decode_attention(const void* q, int64_t q_ld, int64_t rows, int n_q,
                         const uint8_t* v_scale, int64_t n_pages, int page_tokens,
                         const int32_t* table, int64_t table_width,
                         int64_t table_ld, const int32_t* used, float softmax_scale,
-                        void* out, int64_t out_ld, void* q_out, float* scale_out,
+                        void* workspace, int64_t workspace_size, void* out,
+                        int64_t out_ld, void* q_out, float* scale_out,
                         int64_t scale_ld, int ue8m0, float* lse_out, void* stream);
 
 /* Bytes of workspace that qb_beam_select needs for these sizes. */

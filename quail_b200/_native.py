@@ -57,8 +57,10 @@ SIGNATURES = {
                           _I64, _P],
     "qb_kv_quant_read": [_P, _P, _P, _P, _I64, _P, _P, _I64, _I32, _I32, _P, _P, _I64, _I64,
                          _I64, _P],
+    "qb_decode_attention_workspace": [_P],
     "qb_decode_attention": [_P, _I64, _I64, _I32, _I32, _I32, _P, _P, _P, _P, _I64, _I32, _P,
-                            _I64, _I64, _P, _F32, _P, _I64, _P, _P, _I64, _I32, _P, _P],
+                            _I64, _I64, _P, _F32, _P, _I64, _P, _I64, _P, _P, _I64, _I32, _P,
+                            _P],
     "qb_beam_select_workspace": [_I64, _I32, _I64, _I32, _P],
     "qb_beam_select": [_P, _I32, _I64, _I64, _I32, _I64, _P, _P, _I64, _I32, _P, _I64, _P, _P,
                        _P, _P],
@@ -109,7 +111,7 @@ def check(status: int, what: str) -> None:
 # entry points that launch a kernel; LAUNCHES counts them per process
 LAUNCHING = frozenset(n for n in SIGNATURES if n not in (
     "qb_version", "qb_last_error", "qb_kernel_status", "qb_set_wait_limit",
-    "qb_tree_attention_tiles", "qb_beam_select_workspace"))
+    "qb_tree_attention_tiles", "qb_decode_attention_workspace", "qb_beam_select_workspace"))
 LAUNCHES = {"count": 0}
 
 

@@ -18,6 +18,18 @@
 // descriptors; here a lane's 16-byte global loads are the operand fragments
 // themselves (the inner dimension's order is free, so each lane takes the
 // columns that it loaded), and nothing is staged.
+//
+// Split and join. The rows' lengths are known on the device only (a captured
+// launch serves every step), so the blocks share the work there: an item is
+// one row and one tile of 8 query heads, its units are steps of 16 keys, and
+// all items' units laid end to end are cut into as many equal ranges as there
+// are resident blocks, and a block's range into one for each warp. A warp walks
+// its range alone; items that lie within it are finished there, the parts of
+// the others (two a warp at most) meet in shared memory at the block's end,
+// and parts of an item that blocks share in the workspace: the block that
+// completes the item (a counter per cut) joins its parts in the blocks' order,
+// so the result does not depend on who came last. Nothing waits. A block's cut
+// that would part a short item, or leave a sliver, moves to the item's edge.
 #include <cuda_fp16.h>
 
 #include "common.cuh"
@@ -28,12 +40,26 @@ using namespace qb;
 
 constexpr int WARPS = 8;      // of one block; they take a head's key steps in turn
 constexpr int HEADS = 8;      // query heads of a block: the MMA's N
+constexpr int STEP = 16;      // keys of a warp's step, and of a unit of work
+constexpr int BLOCKS_PER_SM = 2;
+constexpr int MIN_UNITS = WARPS;        // a block's least part of an item: a step a warp
+constexpr int WHOLE_UNITS = 2 * WARPS;  // items up to this long are not cut
 constexpr float LN2 = 0.693147180559945309f;
 constexpr float LOG2E = 1.44269504088896341f;
+
+// A part of an item: outputs not yet divided by the sum, per head the
+// exponent they are taken against, the sum, and (8 bit) the outputs' own
+// exponent.
+template <int D>
+struct alignas(16) Part {
+    float o[HEADS][D];
+    float m[HEADS], l[HEADS], mv[HEADS], pad[HEADS];
+};
 
 struct Params {
     const bf16* q;
     int64_t q_ld;
+    int rows;
     int n_q, n_kv, group;             // group = n_q / n_kv
     int tiles;                        // ceil(group / HEADS) blocks share a KV head
     const void* k;
@@ -53,8 +79,33 @@ struct Params {
     int64_t scale_ld;
     bool ue8m0;
     float* lse;
+    void* parts;                      // two Part<D> a block
+    uint32_t* arrived;                // a counter a cut, zero between launches
     uint32_t* status;
 };
+
+// Row r's keys, made to fit its table.
+__device__ __forceinline__ int row_keys(const Params& p, int r, bool flag) {
+    const int n = p.used[r];
+    const int most = (int)(p.table_width << p.page_shift);
+    if (n >= 0 && n <= most) return n;
+    if (flag) atomicOr(p.status, STATUS_BAD_INDEX);
+    return n < 0 ? 0 : most;
+}
+
+// Where a block's range ends: the item there, as its place in the row order.
+struct Cut {
+    int64_t at;       // unit, over all items
+    int64_t before;   // units of the rows before `row`, one head
+    int row;
+};
+
+// The cut x of [0, total) moved off short items and slivers: within the item
+// [s, s + n)
+__device__ __forceinline__ int64_t settle(int64_t x, int64_t s, int n) {
+    if (n <= WHOLE_UNITS || x - s < MIN_UNITS) return s;
+    return s + n - x < MIN_UNITS ? s + n : x;
+}
 
 // 16 (or 8) bytes of the pools: read once, so not kept in L1
 __device__ __forceinline__ uint4 load16(const void* p) {
@@ -117,36 +168,33 @@ __device__ __forceinline__ float e8m0_float(uint32_t b) {
     return __uint_as_float(b ? b << 23 : 0x00400000u);
 }
 
-// One block: one row, one KV head, up to 8 of its query heads. Warp w takes
-// the key steps w, w + 8, ...; the warps' partial results meet in shared
-// memory at the end.
+// A warp's part of an item in shared memory (the padding keeps the rows of
+// neighbouring heads on different banks).
+template <int D>
+struct alignas(16) Slot {
+    float o[HEADS][D + 4];
+    float m[HEADS], l[HEADS], mv[HEADS];
+    int64_t start;       // the item's first unit, over all items; -1: no part
+    int n, row, item;    // its units, row and place in the row
+    int whole;           // 2: starts the item, 1: ends it
+};
+static_assert(sizeof(Slot<64>) % 16 == 0 && sizeof(Slot<128>) % 16 == 0,
+              "the slots' outputs are read as float4");
+
+// One warp: keys [key0, end) of row `row`, KV head kvh, query heads head0 ..
+// head0 + heads - 1; the result to `slot`.
 //
 // Lanes: g = lane / 4, t = lane % 4, as the MMA fragments number them.
 template <int D, bool FP8>
-__global__ void __launch_bounds__(WARPS * 32)
-decode_attention_kernel(const Params p) {
-    constexpr int STEP = 16;                     // keys of a warp's step
+__device__ __forceinline__ void attend(const Params& p, Slot<D>& slot, int row, int kvh,
+                                       int head0, int heads, int key0, int end, int lane) {
     constexpr int ELEM = FP8 ? 1 : 2;
     constexpr int KC = D * ELEM / 64;            // 16-byte chunks of a K row a lane
     constexpr int VC = FP8 ? 1 : D / 64;         // chunks of a V row a lane
     constexpr int MT = D / 16;                   // 16-row tiles of O^T
-    __shared__ float s_o[WARPS][HEADS][D + 4];
-    __shared__ float s_m[WARPS][HEADS], s_l[WARPS][HEADS], s_mv[WARPS][HEADS];
-
-    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     const int g = lane >> 2, t = lane & 3;
-    const int row = blockIdx.y;
-    const int kvh = blockIdx.x / p.tiles, tile = blockIdx.x % p.tiles;
-    const int head0 = kvh * p.group + tile * HEADS;              // first query head
-    const int heads = min(HEADS, p.group - tile * HEADS);
     const int page = 1 << p.page_shift;
     const int32_t* table = p.table + row * p.table_ld;
-
-    int used = p.used[row];
-    if (used < 0 || used > (p.table_width << p.page_shift)) {
-        if (threadIdx.x == 0) atomicOr(p.status, STATUS_BAD_INDEX);
-        used = used < 0 ? 0 : (int)(p.table_width << p.page_shift);
-    }
 
     // Q as the B fragments of S^T: this lane's columns of head g
     uint32_t qf[D / 8];
@@ -220,16 +268,16 @@ decode_attention_kernel(const Params p) {
     const char* k_base = (const char*)p.k + (int64_t)kvh * D * ELEM;
     const char* v_base = (const char*)p.v + (int64_t)kvh * D * ELEM;
 
-    for (int key0 = warp * STEP; key0 < used; key0 += WARPS * STEP) {
+    for (; key0 < end; key0 += STEP) {
         // a page holds a multiple of 8 tokens, so each half step is in one page
         int64_t half_row[2];
         bool half_ok[2];
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
             const int key = key0 + 8 * h;
-            const int id = key < used ? table[key >> p.page_shift] : 0;
-            half_ok[h] = key < used && id >= 0 && id < p.n_pages;
-            if (key < used && !half_ok[h] && lane == 0) atomicOr(p.status, STATUS_BAD_INDEX);
+            const int id = key < end ? table[key >> p.page_shift] : 0;
+            half_ok[h] = key < end && id >= 0 && id < p.n_pages;
+            if (key < end && !half_ok[h] && lane == 0) atomicOr(p.status, STATUS_BAD_INDEX);
             half_row[h] = ((int64_t)(half_ok[h] ? id : 0) << p.page_shift) + (key & (page - 1));
         }
         // ---- K: rows g and g + 8 of the step
@@ -238,7 +286,7 @@ decode_attention_kernel(const Params p) {
         bool k_ok[2];
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
-            k_ok[h] = half_ok[h] && key0 + 8 * h + g < used;
+            k_ok[h] = half_ok[h] && key0 + 8 * h + g < end;
             const int64_t at = half_row[h] + g;
 #pragma unroll
             for (int c = 0; c < KC; ++c)
@@ -253,7 +301,7 @@ decode_attention_kernel(const Params p) {
 #pragma unroll
         for (int r = 0; r < 4; ++r) {
             const int h = r >> 1, off = 2 * t + (r & 1);
-            const bool ok = half_ok[h] && key0 + 8 * h + off < used;
+            const bool ok = half_ok[h] && key0 + 8 * h + off < end;
             const int64_t at = half_row[h] + off;
 #pragma unroll
             for (int c = 0; c < VC; ++c) {
@@ -404,67 +452,81 @@ decode_attention_kernel(const Params p) {
 #pragma unroll
         for (int off = 4; off < 32; off <<= 1)
             sum[n] += __shfl_xor_sync(0xffffffffu, sum[n], off);
+        const int head = 2 * t + n;
         if (g == 0) {
-            s_m[warp][2 * t + n] = top[n] > NEG_INF || sum[n] != 0.0f ? ref[n] : NEG_INF;
-            s_l[warp][2 * t + n] = sum[n];
-            // (a finite x whose value exponent is NaN leaves top_v behind)
-            s_mv[warp][2 * t + n] =
-                top_v[n] > NEG_INF || top[n] > NEG_INF ? ref_v[n] : NEG_INF;
+            // (a NaN product leaves a NaN sum and no maximum, a NaN exponent of
+            // a value leaves top_v behind: both count as parts)
+            slot.m[head] = top[n] > NEG_INF || sum[n] != 0.0f ? ref[n] : NEG_INF;
+            slot.l[head] = sum[n];
+            slot.mv[head] = top_v[n] > NEG_INF || top[n] > NEG_INF ? ref_v[n] : NEG_INF;
         }
 #pragma unroll
-        for (int i = 0; i < MT; ++i)
-#pragma unroll
-            for (int e = 0; e < 2; ++e) {
-                // column of tile i, row g (e = 0) or g + 8 (e = 1)
-                const int d = FP8 ? (D / 8) * g + 2 * i + e
-                                  : 8 * (g + 8 * (i >> 2)) + 2 * (i & 3) + e;
-                s_o[warp][2 * t + n][d] = o[i][2 * e + n];
-            }
+        for (int i = 0; i < MT; i += 2) {   // rows g of tile i, g + 8, and of tile i + 1
+            const int d = FP8 ? (D / 8) * g + 2 * i : 8 * (g + 8 * (i >> 2)) + 2 * (i & 3);
+            *reinterpret_cast<float4*>(&slot.o[head][d]) =
+                make_float4(o[i][n], o[i][2 + n], o[i + 1][n], o[i + 1][2 + n]);
+        }
     }
-    __syncthreads();
+}
 
-    // ---- join: four columns of one head a thread
-    constexpr int QUADS = D / 4;
-    const int head = threadIdx.x / QUADS, d4 = (threadIdx.x % QUADS) * 4;
-    if (head >= HEADS) return;   // D = 64: half of the threads
-    float m = NEG_INF, mv = NEG_INF;
-#pragma unroll
-    for (int i = 0; i < WARPS; ++i) {
-        m = fmaxf(m, s_m[i][head]);
-        mv = fmaxf(mv, s_mv[i][head]);
+// Four columns of one head, as the join accumulates them: parts with their
+// own exponents, brought to the largest.
+template <bool FP8>
+struct Joined {
+    float m, mv, l, acc[4];
+    __device__ __forceinline__ Joined() {
+        m = mv = __uint_as_float(0xFF800000u);
+        l = acc[0] = acc[1] = acc[2] = acc[3] = 0.0f;
     }
-    float l = 0.0f, acc[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-    for (int i = 0; i < WARPS; ++i) {
-        const float mi = s_m[i][head];
-        if (mi > NEG_INF || s_l[i][head] != 0.0f) l += s_l[i][head] * exp2f(mi - m);
-        const float mvi = FP8 ? s_mv[i][head] : mi;
-        if (mvi == NEG_INF) continue;
-        const float f = exp2f(mvi - (FP8 ? mv : m));
-        const float4 part = *reinterpret_cast<const float4*>(&s_o[i][head][d4]);
-        acc[0] += f * part.x;
-        acc[1] += f * part.y;
-        acc[2] += f * part.z;
-        acc[3] += f * part.w;
+    // x against the exponent `from`, brought to `to`; nothing has `from` -inf
+    static __device__ __forceinline__ float factor(float from, float to) {
+        return from > __uint_as_float(0xFF800000u) ? exp2f(from - to) : 0.0f;
     }
+    __device__ __forceinline__ void add(float mi, float li, float mvi, const float4& part) {
+        const float top = fmaxf(m, mi);
+        const float a = factor(m, top), b = factor(mi, top);
+        l = l * a + li * b;
+        m = top;
+        float fa = a, fb = b;
+        if (FP8) {
+            const float top_v = fmaxf(mv, mvi);
+            fa = factor(mv, top_v);
+            fb = factor(mvi, top_v);
+            mv = top_v;
+        }
+        acc[0] = acc[0] * fa + part.x * fb;
+        acc[1] = acc[1] * fa + part.y * fb;
+        acc[2] = acc[2] * fa + part.z * fb;
+        acc[3] = acc[3] * fa + part.w * fb;
+    }
+};
+
+// A head's finished columns d4 .. d4 + 3 to the outputs. D = 128: the 32
+// lanes of a warp hold one head.
+template <int D, bool FP8>
+__device__ __forceinline__ void finish(const Params& p, const Joined<FP8>& j, int row, int head,
+                                       bool live, int d4) {
+    constexpr float LIFT = 13.0f;
+    const float NEG_INF = __uint_as_float(0xFF800000u);
     float r[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-    if (l != 0.0f) {   // a NaN stays one
-        const float f = FP8 && mv > NEG_INF ? exp2f(mv - m - LIFT) : 1.0f;
+    if (j.l != 0.0f) {   // a NaN stays one
+        const float f = FP8 && j.mv > NEG_INF ? exp2f(j.mv - j.m - LIFT) : 1.0f;
 #pragma unroll
-        for (int i = 0; i < 4; ++i) r[i] = acc[i] / l * f;
+        for (int i = 0; i < 4; ++i) r[i] = j.acc[i] / j.l * f;
     }
-    if (head < heads) {
-        const int64_t h = head0 + head;
-        if (p.lse && d4 == 0) p.lse[row * (int64_t)p.n_q + h] = l != 0.0f ? m * LN2 + logf(l) : NEG_INF;
+    if (live) {
+        if (p.lse && d4 == 0)
+            p.lse[row * (int64_t)p.n_q + head] = j.l != 0.0f ? j.m * LN2 + logf(j.l) : NEG_INF;
         if (p.out) {
             uint2 b;
             b.x = bf16x2_bits(r[0], r[1]);
             b.y = bf16x2_bits(r[2], r[3]);
-            *reinterpret_cast<uint2*>(p.out + row * p.out_ld + h * D + d4) = b;
+            *reinterpret_cast<uint2*>(p.out + row * p.out_ld + (int64_t)head * D + d4) = b;
         }
     }
     if (D == 128 && p.q_out) {
         // o_proj's input: bf16 first, then the head's 128 columns as one
-        // quantisation group, as the prefill attention does; a warp holds a head
+        // quantisation group, as the prefill attention does
         float b[4], amax = 0.0f;
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
@@ -474,27 +536,277 @@ decode_attention_kernel(const Params p) {
         amax = warp_max(amax);
         const float scale = p.ue8m0 ? ue8m0_scale(amax) : group_scale(amax);
         const GroupDivider div(scale);
-        if (head < heads) {
-            const int64_t h = head0 + head;
+        if (live) {
             const uint32_t lo = fp8x2(div.quant(b[0]), div.quant(b[1]));
             const uint32_t hi = fp8x2(div.quant(b[2]), div.quant(b[3]));
-            *reinterpret_cast<uint32_t*>(p.q_out + row * (int64_t)p.n_q * D + h * D + d4) =
+            *reinterpret_cast<uint32_t*>(p.q_out + row * (int64_t)p.n_q * D + head * D + d4) =
                 lo | (hi << 16);
-            if (d4 == 0) p.scale_out[h * p.scale_ld + row] = scale;
+            if (d4 == 0) p.scale_out[head * p.scale_ld + row] = scale;
         }
     }
 }
 
+__device__ __forceinline__ int64_t ceil_div(int64_t a, int64_t b) { return (a + b - 1) / b; }
+
+// The row at or after `row` (`before`: one head's units of the rows before it)
+// that holds unit `at`, and its units n. One warp.
+__device__ __forceinline__ void find_row(const Params& p, int64_t at, int per_row, int lane,
+                                         int& row, int64_t& before, int& n) {
+    for (;;) {
+        const int r = row + lane;
+        const int mine = r < p.rows ? (row_keys(p, r, false) + STEP - 1) / STEP : 0;
+        int64_t upto = mine;
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+            const int64_t u = __shfl_up_sync(0xffffffffu, upto, o);
+            if (lane >= o) upto += u;
+        }
+        const uint32_t past = __ballot_sync(0xffffffffu, at < (before + upto) * per_row);
+        const int hit = past ? __ffs(past) - 1 : 31;
+        const int64_t through = __shfl_sync(0xffffffffu, upto, hit);
+        n = __shfl_sync(0xffffffffu, mine, hit);
+        row += hit;
+        before += through - n;
+        if (past || row + 1 >= p.rows) return;
+        before += n;
+        row += 1;
+    }
+}
+
+template <int D, bool FP8>
+__global__ void __launch_bounds__(WARPS * 32, BLOCKS_PER_SM)
+decode_attention_kernel(const Params p) {
+    constexpr int THREADS = WARPS * 32;
+    constexpr int QUADS = D / 4;   // threads of a head in the join
+    extern __shared__ __align__(16) char smem[];
+    Slot<D>* slots = reinterpret_cast<Slot<D>*>(smem);   // [WARPS][2]: begun before, begun here
+    __shared__ int64_t s_scan[WARPS], s_items[WARPS];
+    __shared__ Cut s_cut[2];
+    __shared__ uint32_t s_last;
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+    const int per_row = p.n_kv * p.tiles;   // items of a row
+
+    // ---- this block's range: a scan over the rows' units
+    const int chunk = (p.rows + THREADS - 1) / THREADS;
+    const int r0 = min(tid * chunk, p.rows), r1 = min(r0 + chunk, p.rows);
+    int64_t mine = 0;
+    int full = 0;   // rows that hold keys
+    for (int r = r0; r < r1; ++r) {
+        const int n = (row_keys(p, r, blockIdx.x == 0) + STEP - 1) / STEP;
+        mine += n;
+        full += n > 0;
+    }
+    int64_t upto = mine;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+        const int64_t u = __shfl_up_sync(0xffffffffu, upto, o);
+        if (lane >= o) upto += u;
+    }
+    full = __reduce_add_sync(0xffffffffu, full);
+    if (lane == 31) {
+        s_scan[warp] = upto;
+        s_items[warp] = full;
+    }
+    __syncthreads();
+    int64_t units = 0, items = 0;
+#pragma unroll
+    for (int w = 0; w < WARPS; ++w) {
+        if (w < warp) upto += s_scan[w];
+        units += s_scan[w];
+        items += s_items[w];
+    }
+    const int64_t total = units * per_row;
+    items *= per_row;
+    // a block an item where the items are short, and no block under MIN_UNITS
+    // of a long one
+    const int64_t blocks = min((int64_t)gridDim.x, max(items, total / MIN_UNITS));
+    if ((int64_t)blockIdx.x < blocks) {
+#pragma unroll
+        for (int c = 0; c < 2; ++c) {
+            const int64_t g = (int64_t)blockIdx.x + c;
+            const int64_t x = g == blocks ? total : total * g / blocks;
+            if (g == blocks) {
+                if (tid == 0) s_cut[c].at = total;
+            } else if (x >= (upto - mine) * per_row && x < upto * per_row) {
+                int64_t before = upto - mine;
+                int r = r0, n = 0;
+                for (; r < r1; ++r) {
+                    n = (row_keys(p, r, false) + STEP - 1) / STEP;
+                    if (x < (before + n) * per_row) break;
+                    before += n;
+                }
+                const int64_t s = before * per_row + (x - before * per_row) / n * n;
+                s_cut[c].at = settle(x, s, n);
+                s_cut[c].before = before;
+                s_cut[c].row = r;
+            }
+        }
+    }
+    // rows without keys
+    for (int r = blockIdx.x; r < p.rows; r += gridDim.x) {
+        if (row_keys(p, r, false) != 0) continue;
+        const Joined<FP8> none;
+        for (int i = tid; i < p.n_q * QUADS; i += THREADS)
+            finish<D, FP8>(p, none, r, i / QUADS, true, i % QUADS * 4);
+    }
+    if ((int64_t)blockIdx.x >= blocks) return;
+    __syncthreads();
+    const int64_t lo = s_cut[0].at, hi = s_cut[1].at;
+
+    // ---- this warp's range
+    if (lane < 2) slots[2 * warp + lane].start = -1;
+    __syncwarp();
+    int64_t at = lo + (hi - lo) * warp / WARPS;
+    const int64_t end = lo + (hi - lo) * (warp + 1) / WARPS;
+    int row = s_cut[0].row, n = 0;
+    int64_t before = s_cut[0].before;
+    while (at < end) {
+        if (at >= (before + n) * per_row || n == 0) find_row(p, at, per_row, lane, row, before, n);
+        const int item = (int)(at - before * per_row) / n;
+        const int64_t s = before * per_row + (int64_t)item * n;
+        const int64_t stop = min(end, s + n);
+        const int kvh = item / p.tiles, tile = item % p.tiles;
+        const int head0 = kvh * p.group + tile * HEADS;
+        const int heads = min(HEADS, p.group - tile * HEADS);
+        const int whole = 2 * (at == s) + (stop == s + n);
+        Slot<D>& slot = slots[2 * warp + (at == s)];
+        attend<D, FP8>(p, slot, row, kvh, head0, heads, (int)(at - s) * STEP,
+                       min(row_keys(p, row, false), (int)(stop - s) * STEP), lane);
+        __syncwarp();
+        if (whole == 3) {
+            for (int i = lane; i < HEADS * QUADS; i += 32) {
+                const int head = i / QUADS, d4 = i % QUADS * 4;
+                if (D == 128 && head >= heads) break;   // D = 64: two heads at a time
+                Joined<FP8> j;
+                j.add(slot.m[head], slot.l[head], slot.mv[head],
+                      *reinterpret_cast<const float4*>(&slot.o[head][d4]));
+                finish<D, FP8>(p, j, row, head0 + head, head < heads, d4);
+            }
+        } else if (lane == 0) {
+            slot.start = s;
+            slot.n = n;
+            slot.row = row;
+            slot.item = item;
+            slot.whole = whole;
+        }
+        __syncwarp();
+        at = stop;
+    }
+    __syncthreads();
+
+    // ---- the parts that warps share, in order
+    const int my_head = tid / QUADS, d4 = tid % QUADS * 4;
+    const bool have = my_head < HEADS;   // D = 64 leaves half of the threads over
+    for (int i = 0; i < 2 * WARPS;) {
+        const int64_t s = slots[i].start;
+        if (s < 0) {
+            ++i;
+            continue;
+        }
+        const int row = slots[i].row, item = slots[i].item;
+        const int64_t n = slots[i].n;
+        const int kvh = item / p.tiles, tile = item % p.tiles;
+        const int head0 = kvh * p.group + tile * HEADS;
+        const int heads = min(HEADS, p.group - tile * HEADS);
+        const bool begins = slots[i].whole & 2;
+        bool ends = false;
+        Joined<FP8> j;
+        for (; i < 2 * WARPS; ++i) {
+            const Slot<D>& slot = slots[i];
+            if (slot.start < 0) continue;
+            if (slot.start != s) break;
+            ends = slot.whole & 1;
+            if (have)
+                j.add(slot.m[my_head], slot.l[my_head], slot.mv[my_head],
+                      *reinterpret_cast<const float4*>(&slot.o[my_head][d4]));
+        }
+        bool whole = begins && ends;
+        if (!whole) {
+            Part<D>* parts = (Part<D>*)p.parts;
+            Part<D>& part = parts[2 * blockIdx.x + begins];
+            if (have) {
+                __stcg(reinterpret_cast<float4*>(&part.o[my_head][d4]),
+                       make_float4(j.acc[0], j.acc[1], j.acc[2], j.acc[3]));
+                if (d4 == 0) {
+                    __stcg(&part.m[my_head], j.m);
+                    __stcg(&part.l[my_head], j.l);
+                    __stcg(&part.mv[my_head], j.mv);
+                }
+            }
+            // the cuts inside the item, and so the blocks that share it
+            const int64_t first = ceil_div((s + MIN_UNITS) * blocks, total);
+            const int64_t last = ceil_div((s + n - MIN_UNITS + 1) * blocks, total) - 1;
+            __threadfence();
+            __syncthreads();
+            if (tid == 0) {
+                const uint32_t others = atomicAdd(p.arrived + first, 1u);
+                s_last = others == (uint32_t)(last - first + 1);
+                if (s_last) p.arrived[first] = 0;   // for the next launch
+            }
+            __syncthreads();
+            whole = s_last;
+            if (whole && have) {
+                __threadfence();
+                j = Joined<FP8>();
+                for (int64_t b = first - 1; b <= last; ++b) {
+                    const Part<D>& q = parts[2 * b + (b == first - 1)];
+                    j.add(__ldcg(&q.m[my_head]), __ldcg(&q.l[my_head]), __ldcg(&q.mv[my_head]),
+                          __ldcg(reinterpret_cast<const float4*>(&q.o[my_head][d4])));
+                }
+            }
+        }
+        if (whole && have) finish<D, FP8>(p, j, row, head0 + my_head, my_head < heads, d4);
+    }
+}
+
+template <int D, bool FP8>
+int launch(const Params& p, int blocks, cudaStream_t stream) {
+    static std::atomic<bool> done[MAX_DEVICES];
+    constexpr int bytes = 2 * WARPS * sizeof(Slot<D>);
+    if (!set_smem_once(done, decode_attention_kernel<D, FP8>, bytes))
+        return launch_status("qb_decode_attention: shared memory");
+    decode_attention_kernel<D, FP8><<<blocks, WARPS * 32, bytes, stream>>>(p);
+    return launch_status("qb_decode_attention");
+}
+
+// Resident blocks of the current device (0: the query failed).
+int resident_blocks() {
+    static std::atomic<int> cache[MAX_DEVICES];
+    int dev = 0;
+    if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= MAX_DEVICES) return 0;
+    int n = cache[dev].load(std::memory_order_acquire);
+    if (n == 0) {
+        int sms = 0;
+        if (cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess)
+            return 0;
+        n = sms * BLOCKS_PER_SM;
+        cache[dev].store(n, std::memory_order_release);
+    }
+    return n;
+}
+
+int64_t workspace_bytes(int blocks) {
+    return (int64_t)blocks * 2 * sizeof(Part<128>) + (blocks + 1) * (int64_t)sizeof(uint32_t);
+}
+
 }  // namespace
+
+extern "C" int qb_decode_attention_workspace(int64_t* bytes) {
+    if (!bytes) return invalid("qb_decode_attention_workspace: bytes is NULL");
+    const int blocks = resident_blocks();
+    if (!blocks) return launch_status("qb_decode_attention_workspace");
+    *bytes = workspace_bytes(blocks);
+    return QB_OK;
+}
 
 extern "C" int qb_decode_attention(const void* q, int64_t q_ld, int64_t rows, int n_q, int n_kv,
                                    int head_dim, const void* k_pool, const void* v_pool,
                                    const uint8_t* k_scale, const uint8_t* v_scale,
                                    int64_t n_pages, int page_tokens, const int32_t* table,
                                    int64_t table_width, int64_t table_ld, const int32_t* used,
-                                   float softmax_scale, void* out, int64_t out_ld, void* q_out,
-                                   float* scale_out, int64_t scale_ld, int ue8m0, float* lse_out,
-                                   void* stream) {
+                                   float softmax_scale, void* workspace, int64_t workspace_size,
+                                   void* out, int64_t out_ld, void* q_out, float* scale_out,
+                                   int64_t scale_ld, int ue8m0, float* lse_out, void* stream) {
     const char* who = "qb_decode_attention";
     if (head_dim != 64 && head_dim != 128)
         return invalid("qb_decode_attention: head_dim must be 64 or 128");
@@ -524,9 +836,17 @@ extern "C" int qb_decode_attention(const void* q, int64_t q_ld, int64_t rows, in
     if (n_pages <= 0 || table_width <= 0 || table_ld < table_width ||
         table_width > 0x7fffffffLL / page_tokens)
         return invalid("qb_decode_attention: bad table width or page count");
+    if (!workspace || !aligned(workspace, 16))
+        return invalid("qb_decode_attention: the workspace must be 16-byte aligned");
+    const int blocks = resident_blocks();
+    if (!blocks) return launch_status(who);
+    if (workspace_size < workspace_bytes(blocks))
+        return invalid("qb_decode_attention: the workspace is too small "
+                       "(qb_decode_attention_workspace)");
     Params p;
     p.q = (const bf16*)q;
     p.q_ld = q_ld;
+    p.rows = (int)rows;
     p.n_q = n_q;
     p.n_kv = n_kv;
     p.group = n_q / n_kv;
@@ -551,11 +871,10 @@ extern "C" int qb_decode_attention(const void* q, int64_t q_ld, int64_t rows, in
     p.lse = lse_out;
     p.status = device_status_ptr();
     if (!p.status) return launch_status("qb_decode_attention: status word");
-    const dim3 grid((unsigned)(n_kv * p.tiles), (unsigned)rows);
-    auto* kernel = head_dim == 128 ? (k_scale ? decode_attention_kernel<128, true>
-                                              : decode_attention_kernel<128, false>)
-                                   : (k_scale ? decode_attention_kernel<64, true>
-                                              : decode_attention_kernel<64, false>);
-    kernel<<<grid, WARPS * 32, 0, (cudaStream_t)stream>>>(p);
-    return launch_status(who);
+    p.parts = workspace;
+    p.arrived = (uint32_t*)((char*)workspace + (int64_t)blocks * 2 * sizeof(Part<128>));
+    const cudaStream_t st = (cudaStream_t)stream;
+    if (head_dim == 128)
+        return k_scale ? launch<128, true>(p, blocks, st) : launch<128, false>(p, blocks, st);
+    return k_scale ? launch<64, true>(p, blocks, st) : launch<64, false>(p, blocks, st);
 }

@@ -14,6 +14,7 @@ caching allocator unless they are passed in. Shapes and types are checked
 here (ValueError); sizes, strides and alignment by the library.
 """
 
+import ctypes
 from typing import NamedTuple
 
 import torch
@@ -57,52 +58,68 @@ class QuantKV:
         return self.codes, self.scales
 
 
-def _stream(device):
-    return torch.cuda.current_stream(device).cuda_stream
+def _launch(name, device, *args):
+    """One library call on the current stream of CUDA device `device`."""
+    stream = torch._C._cuda_getCurrentRawStream(device)
+    if device == torch._C._cuda_getDevice():
+        nat.call(name, *args, stream)
+    else:
+        with torch.cuda.device(device):
+            nat.call(name, *args, stream)
 
 
-def _need(ok, what):
-    if not ok:
-        raise ValueError(what)
-
-
-def _same_device(who, first, *tensors):
-    for t in tensors:
-        if t is not None and t.device != first.device:
-            raise ValueError(f"{who}: tensors on different devices")
-    if first.device.type != "cuda":
+def _device(who, *tensors):
+    """The index of the one CUDA device that holds the tensors (None skipped)."""
+    device = tensors[0].get_device()
+    if device < 0:
         raise ValueError(f"{who}: CUDA tensors are needed")
+    for t in tensors:
+        if t is not None and t.get_device() != device:
+            raise ValueError(f"{who}: tensors on different devices")
+    return device
 
 
-def _heads(who, name, x, n_kv=None, d=None):
-    """x as bf16 rows of heads [rows, n, d], each row's heads contiguous."""
-    _need(x.dim() == 3 and x.dtype == torch.bfloat16, f"{who}: {name} must be bf16 [rows, n, d]")
-    _need(n_kv is None or (x.shape[1] == n_kv and x.shape[2] == d),
-          f"{who}: {name}'s heads are not the cache's")
-    _need(x.stride(2) == 1 and (x.shape[1] == 1 or x.stride(1) == x.shape[2]),
-          f"{who}: the heads of a row of {name} must be contiguous")
-
-
-def _row_stride(x):
+def _heads(who, name, x):
+    """(rows, heads, d, row stride) of bf16 rows of heads [rows, n, d], each
+    row's heads contiguous."""
+    if x.dim() != 3 or x.dtype != torch.bfloat16:
+        raise ValueError(f"{who}: {name} must be bf16 [rows, n, d]")
+    rows, n, d = x.shape
+    ld, head, one = x.stride()
+    if one != 1 or (head != d and n > 1):
+        raise ValueError(f"{who}: the heads of a row of {name} must be contiguous")
     # a single row's stride may be anything; the library wants one that covers it
-    return x.stride(0) if x.shape[0] > 1 else -(-x.shape[1] * x.shape[2] // 8) * 8
+    return rows, n, d, ld if rows > 1 else -(-n * d // 8) * 8
 
 
 def _quant_layer(who, kv):
-    rows, n_kv, d = kv.k.shape
-    for c, s in ((kv.k, kv.k_scale), (kv.v, kv.v_scale)):
-        _need(c.shape == (rows, n_kv, d) and s.shape == (rows, n_kv)
-              and c.dtype == torch.float8_e4m3fn and s.dtype == torch.uint8
-              and c.is_contiguous() and s.is_contiguous(),
-              f"{who}: the cache needs contiguous e4m3 codes [rows, n_kv, d] and uint8 scales "
-              f"[rows, n_kv]")
-    return rows, n_kv, d
+    k, v, ks, vs = kv
+    shape = k.shape
+    if not (len(shape) == 3 and v.shape == shape and ks.shape == vs.shape == shape[:2]
+            and k.dtype == v.dtype == torch.float8_e4m3fn
+            and ks.dtype == vs.dtype == torch.uint8
+            and k.is_contiguous() and v.is_contiguous()
+            and ks.is_contiguous() and vs.is_contiguous()):
+        raise ValueError(f"{who}: the cache needs contiguous e4m3 codes [rows, n_kv, d] and "
+                         "uint8 scales [rows, n_kv]")
+    return shape
 
 
 def _index(who, name, x, n=None):
-    _need(x.dtype == torch.int64 and x.dim() == 1 and x.is_contiguous()
-          and (n is None or x.shape[0] == n), f"{who}: {name} must be a contiguous int64 vector "
-          "as long as the rows")
+    if x.dtype != torch.int64 or x.dim() != 1 or not x.is_contiguous() or (
+            n is not None and x.shape[0] != n):
+        raise ValueError(f"{who}: {name} must be a contiguous int64 vector as long as the rows")
+
+
+def _rows_of(who, k, v, n_kv, d):
+    """(rows, k's and v's row strides) of bf16 K and V of the cache's heads."""
+    rows, n, width, k_ld = _heads(who, "k", k)
+    v_rows, n_v, v_width, v_ld = _heads(who, "v", v)
+    if n != n_kv or n_v != n_kv or width != d or v_width != d:
+        raise ValueError(f"{who}: the heads of k and v are not the cache's")
+    if rows != v_rows:
+        raise ValueError(f"{who}: k and v differ in rows")
+    return rows, k_ld, v_ld
 
 
 def kv_quant_write(k, v, kv: QuantLayer, dst, src=None):
@@ -115,17 +132,16 @@ def kv_quant_write(k, v, kv: QuantLayer, dst, src=None):
     """
     who = "kv_quant_write"
     pool_rows, n_kv, d = _quant_layer(who, kv)
-    _heads(who, "k", k, n_kv, d)
-    _heads(who, "v", v, n_kv, d)
-    _need(k.shape == v.shape, f"{who}: k and v differ in rows")
-    _index(who, "dst", dst, k.shape[0] if src is None else src.shape[0])
+    rows, k_ld, v_ld = _rows_of(who, k, v, n_kv, d)
     if src is not None:
         _index(who, "src", src)
-    _same_device(who, k, v, dst, src, *kv)
-    nat.call("qb_kv_quant_write", k.data_ptr(), v.data_ptr(), _row_stride(k), _row_stride(v),
-             None if src is None else src.data_ptr(), dst.data_ptr(), dst.shape[0], k.shape[0],
-             n_kv, d, kv.k.data_ptr(), kv.v.data_ptr(), kv.k_scale.data_ptr(),
-             kv.v_scale.data_ptr(), pool_rows, _stream(k.device))
+    n = rows if src is None else src.shape[0]
+    _index(who, "dst", dst, n)
+    device = _device(who, k, v, dst, src, *kv)
+    _launch("qb_kv_quant_write", device, k.data_ptr(), v.data_ptr(), k_ld, v_ld,
+            None if src is None else src.data_ptr(), dst.data_ptr(), n, rows, n_kv, d,
+            kv.k.data_ptr(), kv.v.data_ptr(), kv.k_scale.data_ptr(), kv.v_scale.data_ptr(),
+            pool_rows)
 
 
 def kv_quant_read(kv: QuantLayer, src, dst=None, out=None):
@@ -138,48 +154,52 @@ def kv_quant_read(kv: QuantLayer, src, dst=None, out=None):
     _index(who, "src", src)
     n = src.shape[0]
     if out is None:
-        _need(dst is None, f"{who}: dst needs out")
-        k = torch.empty((n, n_kv, d), dtype=torch.bfloat16, device=kv.k.device)
-        v = torch.empty_like(k)
+        if dst is not None:
+            raise ValueError(f"{who}: dst needs out")
+        k, v = kv.k.new_empty((2, n, n_kv, d), dtype=torch.bfloat16).unbind(0)
+        rows, k_ld, v_ld = n, n_kv * d, n_kv * d
     else:
         k, v = out
-        _heads(who, "k", k, n_kv, d)
-        _heads(who, "v", v, n_kv, d)
-        _need(k.shape == v.shape, f"{who}: k and v differ in rows")
-    if dst is not None:
-        _index(who, "dst", dst, n)
-    _same_device(who, kv.k, k, v, src, dst, *kv)
-    nat.call("qb_kv_quant_read", kv.k.data_ptr(), kv.v.data_ptr(), kv.k_scale.data_ptr(),
-             kv.v_scale.data_ptr(), pool_rows, src.data_ptr(),
-             None if dst is None else dst.data_ptr(), n, n_kv, d, k.data_ptr(), v.data_ptr(),
-             _row_stride(k), _row_stride(v), k.shape[0], _stream(k.device))
+        rows, k_ld, v_ld = _rows_of(who, k, v, n_kv, d)
+        if dst is not None:
+            _index(who, "dst", dst, n)
+    device = _device(who, k, v, src, dst, *kv)
+    _launch("qb_kv_quant_read", device, kv.k.data_ptr(), kv.v.data_ptr(),
+            kv.k_scale.data_ptr(), kv.v_scale.data_ptr(), pool_rows, src.data_ptr(),
+            None if dst is None else dst.data_ptr(), n, n_kv, d, k.data_ptr(), v.data_ptr(),
+            k_ld, v_ld, rows)
     return k, v
 
 
-def _decode_args(who, q, kv, table, used, page_tokens):
-    _heads(who, "q", q)
-    if isinstance(kv, QuantLayer):
-        pool_rows, n_kv, d = _quant_layer(who, kv)
-        k, v, ks, vs = kv
-    else:
-        k, v = kv
-        ks = vs = None
-        _need(k.dim() == 3 and k.shape == v.shape and k.dtype == v.dtype == torch.bfloat16
-              and k.is_contiguous() and v.is_contiguous(),
-              f"{who}: bf16 pools must be contiguous [rows, n_kv, d]")
-        pool_rows, n_kv, d = k.shape
-    _need(q.shape[2] == d, f"{who}: q's head size is not the cache's")
-    _need(pool_rows % page_tokens == 0, f"{who}: the pools are not whole pages")
-    _need(table.dim() == 2 and table.dtype == torch.int32 and table.shape[0] == q.shape[0]
-          and table.stride(1) == 1, f"{who}: table must be int32 [rows, pages]")
-    _need(used.dim() == 1 and used.dtype == torch.int32 and used.shape[0] == q.shape[0]
-          and used.is_contiguous(), f"{who}: used must be int32 [rows]")
-    _same_device(who, q, k, v, ks, vs, table, used)
-    return k, v, ks, vs, pool_rows, n_kv, d
+_workspaces = {}   # (device, stream) -> the attention's workspace there
+
+
+def decode_workspace(device="cuda"):
+    """A workspace for decode_attention calls that follow one another (one
+    stream, one captured graph): its size does not depend on a call's, and each
+    call leaves it as it found it."""
+    with torch.cuda.device(device):
+        need = ctypes.c_int64(0)
+        nat.call("qb_decode_attention_workspace", ctypes.byref(need))
+        return torch.zeros(need.value, dtype=torch.uint8, device="cuda")
+
+
+def _stream_workspace(device):
+    """The current stream's own workspace, kept. A graph that is being captured
+    must not share it (the graph may be replayed beside the stream), so there a
+    call gets a fresh one, whose zeroing the graph repeats: pass workspace= to
+    spare that."""
+    if torch.cuda.is_current_stream_capturing():
+        return decode_workspace(device)
+    stream = torch._C._cuda_getCurrentRawStream(device)
+    held = _workspaces.get((device, stream))
+    if held is None:
+        held = _workspaces[device, stream] = decode_workspace(device)
+    return held
 
 
 def decode_attention(q, kv, table, used, *, page_tokens=16, softmax_scale=None, out=None,
-                     with_lse=False, quantised=None):
+                     with_lse=False, quantised=None, workspace=None):
     """Attention of one new token per row over its paged KV cache.
 
     q: bf16 [rows, n_q, d]; kv: an arena's (k, v) pools of one layer (bf16
@@ -190,35 +210,63 @@ def decode_attention(q, kv, table, used, *, page_tokens=16, softmax_scale=None, 
     [rows, n_q]. quantised: an engine.QuantRows to fill with the output
     quantised per head (d = 128), in place of the bf16 output unless out is
     given too; the library's UE8M0 mode when it is a (QuantRows, True) pair.
+    workspace: from decode_workspace, for calls that never overlap; the current
+    stream's own when None.
     """
     who = "decode_attention"
-    k, v, ks, vs, pool_rows, n_kv, d = _decode_args(who, q, kv, table, used, page_tokens)
-    rows, n_q = q.shape[0], q.shape[1]
-    ue8m0 = False
-    if isinstance(quantised, tuple):
-        quantised, ue8m0 = quantised
-    if out is None and quantised is None:
-        out = torch.empty((rows, n_q, d), dtype=torch.bfloat16, device=q.device)
-    elif out is not None:
-        _heads(who, "out", out)
-        _need(out.shape == q.shape, f"{who}: out must have q's shape")
-        _same_device(who, q, out)
+    rows, n_q, d, q_ld = _heads(who, "q", q)
+    if len(kv) == 4:
+        pool_rows, n_kv, width = _quant_layer(who, kv)
+        k, v, ks, vs = kv
+    else:
+        k, v = kv
+        ks = vs = None
+        if not (k.dim() == 3 and k.shape == v.shape and k.dtype == v.dtype == torch.bfloat16
+                and k.is_contiguous() and v.is_contiguous()):
+            raise ValueError(f"{who}: bf16 pools must be contiguous [rows, n_kv, d]")
+        pool_rows, n_kv, width = k.shape
+    if width != d:
+        raise ValueError(f"{who}: q's head size is not the cache's")
+    if pool_rows % page_tokens:
+        raise ValueError(f"{who}: the pools are not whole pages")
+    if table.dim() != 2 or table.dtype != torch.int32 or table.shape[0] != rows or (
+            table.stride(1) != 1):
+        raise ValueError(f"{who}: table must be int32 [rows, pages]")
+    if used.dim() != 1 or used.dtype != torch.int32 or used.shape[0] != rows or (
+            not used.is_contiguous()):
+        raise ValueError(f"{who}: used must be int32 [rows]")
+    q8 = q8_scale = None
+    q8_ld, ue8m0, out_ld = 0, False, 0
     if quantised is not None:
-        _need(quantised.q.shape == (rows, n_q * d) and quantised.q.is_contiguous()
-              and quantised.scale.shape[0] == n_q and quantised.scale.is_contiguous(),
-              f"{who}: quantised must hold [rows, n_q * d] codes and [n_q, ld] scales")
-        _same_device(who, q, quantised.q, quantised.scale)
-    lse = torch.empty((rows, n_q), dtype=torch.float32, device=q.device) if with_lse else None
-    nat.call("qb_decode_attention", q.data_ptr(), _row_stride(q), rows, n_q, n_kv, d,
-             k.data_ptr(), v.data_ptr(), None if ks is None else ks.data_ptr(),
-             None if vs is None else vs.data_ptr(), pool_rows // page_tokens, page_tokens,
-             table.data_ptr(), table.shape[1], table.stride(0) if rows > 1 else table.shape[1],
-             used.data_ptr(), d ** -0.5 if softmax_scale is None else softmax_scale,
-             None if out is None else out.data_ptr(), 0 if out is None else _row_stride(out),
-             None if quantised is None else quantised.q.data_ptr(),
-             None if quantised is None else quantised.scale.data_ptr(),
-             0 if quantised is None else quantised.ld, int(ue8m0),
-             None if lse is None else lse.data_ptr(), _stream(q.device))
+        if isinstance(quantised, tuple):
+            quantised, ue8m0 = quantised
+        q8, q8_scale, q8_ld = quantised.q, quantised.scale, quantised.ld
+        if not (q8.shape == (rows, n_q * d) and q8.is_contiguous()
+                and q8_scale.shape[0] == n_q and q8_scale.is_contiguous()):
+            raise ValueError(f"{who}: quantised must hold [rows, n_q * d] codes and [n_q, ld] "
+                             "scales")
+    if out is not None:
+        if out.shape != q.shape:
+            raise ValueError(f"{who}: out must have q's shape")
+        out_ld = _heads(who, "out", out)[3]
+    device = _device(who, q, k, v, ks, vs, table, used, out, q8, q8_scale, workspace)
+    if out is None and q8 is None:
+        out = q.new_empty((rows, n_q, d))
+        out_ld = n_q * d
+    lse = q.new_empty((rows, n_q), dtype=torch.float32) if with_lse else None
+    table_width = table.shape[1]
+    if workspace is None:
+        workspace = _stream_workspace(device)
+    _launch("qb_decode_attention", device, q.data_ptr(), q_ld, rows, n_q, n_kv, d, k.data_ptr(),
+            v.data_ptr(), None if ks is None else ks.data_ptr(),
+            None if vs is None else vs.data_ptr(), pool_rows // page_tokens, page_tokens,
+            table.data_ptr(), table_width, table.stride(0) if rows > 1 else table_width,
+            used.data_ptr(), d ** -0.5 if softmax_scale is None else softmax_scale,
+            workspace.data_ptr(), workspace.shape[0],
+            None if out is None else out.data_ptr(), out_ld,
+            None if q8 is None else q8.data_ptr(),
+            None if q8 is None else q8_scale.data_ptr(), q8_ld, ue8m0,
+            None if lse is None else lse.data_ptr())
     result = quantised if out is None else out
     return (result, lse) if with_lse else result
 
@@ -234,32 +282,32 @@ def beam_select(logits, scores, *, finished=None, pad=0, n_out=None):
     in its group.
     """
     who = "beam_select"
-    _need(scores.dim() == 2 and scores.dtype == torch.float32 and scores.is_contiguous(),
-          f"{who}: scores must be contiguous f32 [groups, beams]")
+    if scores.dim() != 2 or scores.dtype != torch.float32 or not scores.is_contiguous():
+        raise ValueError(f"{who}: scores must be contiguous f32 [groups, beams]")
     groups, beams = scores.shape
     n_out = beams if n_out is None else n_out
-    _need(logits.dim() == 2 and logits.shape[0] == groups * beams
-          and logits.dtype in (torch.float32, torch.bfloat16) and logits.stride(1) == 1,
-          f"{who}: logits must be f32 or bf16 [groups * beams, vocab]")
-    if finished is not None:
-        _need(finished.shape == scores.shape and finished.is_contiguous()
-              and finished.dtype in (torch.bool, torch.uint8),
-              f"{who}: finished must be contiguous bool or uint8 [groups, beams]")
-    _same_device(who, logits, scores, finished)
+    dtype = logits.dtype
+    if logits.dim() != 2 or logits.shape[0] != groups * beams or logits.stride(1) != 1 or (
+            dtype != torch.float32 and dtype != torch.bfloat16):
+        raise ValueError(f"{who}: logits must be f32 or bf16 [groups * beams, vocab]")
+    if finished is not None and not (
+            finished.shape == scores.shape and finished.is_contiguous()
+            and finished.dtype in (torch.bool, torch.uint8)):
+        raise ValueError(f"{who}: finished must be contiguous bool or uint8 [groups, beams]")
+    device = _device(who, logits, scores, finished)
     vocab = logits.shape[1]
-    need = nat.ctypes.c_int64(0)
-    nat.call("qb_beam_select_workspace", groups, beams, vocab, n_out, nat.ctypes.byref(need))
-    dev = logits.device
-    workspace = torch.empty(max(need.value, 16), dtype=torch.uint8, device=dev)
-    out = (torch.empty((groups, n_out), dtype=torch.float32, device=dev),
-           torch.empty((groups, n_out), dtype=torch.int32, device=dev),
-           torch.empty((groups, n_out), dtype=torch.int64, device=dev))
-    nat.call("qb_beam_select", logits.data_ptr(), int(logits.dtype == torch.bfloat16),
-             logits.stride(0) if logits.shape[0] > 1 else vocab, groups, beams, vocab,
-             scores.data_ptr(), None if finished is None else finished.data_ptr(), pad, n_out,
-             workspace.data_ptr(), workspace.shape[0], out[0].data_ptr(), out[1].data_ptr(),
-             out[2].data_ptr(), _stream(dev))
-    return out
+    need = ctypes.c_int64(0)
+    nat.call("qb_beam_select_workspace", groups, beams, vocab, n_out, ctypes.byref(need))
+    workspace = logits.new_empty(max(need.value, 16), dtype=torch.uint8)
+    score = scores.new_empty((groups, n_out))
+    parent = scores.new_empty((groups, n_out), dtype=torch.int32)
+    token = scores.new_empty((groups, n_out), dtype=torch.int64)
+    _launch("qb_beam_select", device, logits.data_ptr(), dtype == torch.bfloat16,
+            logits.stride(0) if groups * beams > 1 else vocab, groups, beams, vocab,
+            scores.data_ptr(), None if finished is None else finished.data_ptr(), pad, n_out,
+            workspace.data_ptr(), need.value, score.data_ptr(), parent.data_ptr(),
+            token.data_ptr())
+    return score, parent, token
 
 
 def beam_reorder(pools, parents, used, table, *, page_tokens=16):
@@ -275,28 +323,32 @@ def beam_reorder(pools, parents, used, table, *, page_tokens=16):
     row of each beam's next token (-1 when its table is full).
     """
     who = "beam_reorder"
-    _need(parents.dim() == 2 and parents.dtype == torch.int32 and parents.is_contiguous(),
-          f"{who}: parents must be contiguous int32 [groups, beams]")
+    if parents.dim() != 2 or parents.dtype != torch.int32 or not parents.is_contiguous():
+        raise ValueError(f"{who}: parents must be contiguous int32 [groups, beams]")
     groups, beams = parents.shape
-    _need(used.shape == (groups,) and used.dtype == torch.int32 and used.is_contiguous(),
-          f"{who}: used must be int32 [groups]")
-    _need(table.dim() == 2 and table.dtype == torch.int32 and table.is_contiguous()
-          and table.shape[0] == groups * beams,
-          f"{who}: table must be contiguous int32 [groups * beams, pages]")
-    _need(len(pools) in (1, 2), f"{who}: one pool, or codes and scales")
-    rows = pools[0].shape[2]
-    _need(rows % page_tokens == 0, f"{who}: the pools are not whole pages")
-    row_bytes = [0, 0]
-    for i, pool in enumerate(pools):
-        _need(pool.dim() >= 4 and pool.shape[:3] == pools[0].shape[:3] and pool.is_contiguous(),
-              f"{who}: pools must be contiguous [n_layers, 2, rows, ...]")
-        row_bytes[i] = pool.stride(2) * pool.element_size()
-    _same_device(who, pools[0], parents, used, table, *pools[1:])
+    if used.dim() != 1 or used.shape[0] != groups or used.dtype != torch.int32 or (
+            not used.is_contiguous()):
+        raise ValueError(f"{who}: used must be int32 [groups]")
+    if table.dim() != 2 or table.dtype != torch.int32 or table.shape[0] != groups * beams or (
+            not table.is_contiguous()):
+        raise ValueError(f"{who}: table must be contiguous int32 [groups * beams, pages]")
+    if len(pools) not in (1, 2):
+        raise ValueError(f"{who}: one pool, or codes and scales")
+    pool = pools[0]
+    second = pools[1] if len(pools) == 2 else None
+    for x in pools:
+        if x.dim() < 4 or x.shape[:3] != pool.shape[:3] or not x.is_contiguous():
+            raise ValueError(f"{who}: pools must be contiguous [n_layers, 2, rows, ...]")
+    layers, two, rows = pool.shape[:3]
+    if rows % page_tokens:
+        raise ValueError(f"{who}: the pools are not whole pages")
+    device = _device(who, pool, second, parents, used, table)
     out = torch.empty_like(table)
-    next_row = torch.empty(groups * beams, dtype=torch.int64, device=table.device)
-    nat.call("qb_beam_reorder", parents.data_ptr(), used.data_ptr(), groups, beams,
-             table.data_ptr(), table.shape[1], page_tokens, rows // page_tokens,
-             pools[0].data_ptr(), pools[0].shape[0] * pools[0].shape[1], row_bytes[0],
-             pools[1].data_ptr() if len(pools) > 1 else None, row_bytes[1], out.data_ptr(),
-             next_row.data_ptr(), _stream(table.device))
+    next_row = table.new_empty(groups * beams, dtype=torch.int64)
+    _launch("qb_beam_reorder", device, parents.data_ptr(), used.data_ptr(), groups, beams,
+            table.data_ptr(), table.shape[1], page_tokens, rows // page_tokens, pool.data_ptr(),
+            layers * two, pool.stride(2) * pool.element_size(),
+            None if second is None else second.data_ptr(),
+            0 if second is None else second.stride(2) * second.element_size(), out.data_ptr(),
+            next_row.data_ptr())
     return out, next_row

@@ -51,7 +51,7 @@ def test_kv_quant_read_refuses(change, match):
 
 ATTN = dict(q=OK, q_ld=1024, rows=4, n_q=8, n_kv=2, d=128, k=OK, v=OK, ks=None, vs=None,
             n_pages=8, page=16, table=OK, width=4, table_ld=4, used=OK, scale=0.1)
-ATTN_OUT = dict(out=OK, out_ld=1024, q_out=None, scale_out=None, scale_ld=0, ue8m0=0, lse=None,
+ATTN_OUT = dict(ws=OK, ws_bytes=1 << 30, out=OK, out_ld=1024, q_out=None, scale_out=None, scale_ld=0, ue8m0=0, lse=None,
                 stream=None)
 
 
@@ -62,6 +62,7 @@ ATTN_OUT = dict(out=OK, out_ld=1024, q_out=None, scale_out=None, scale_ld=0, ue8
     (dict(out_ld=1000), "out_ld"), (dict(table=None), "NULL"), (dict(ks=OK), "together"),
     (dict(k=OFF), "aligned"), (dict(width=0), "width"), (dict(table_ld=3), "width"),
     (dict(n_pages=0), "width"), (dict(width=1 << 40), "width"),
+    (dict(ws=None), "workspace"), (dict(ws=OFF), "workspace"),
     (dict(q_out=OK), "fp8 output"), (dict(q_out=OK, scale_out=OK, scale_ld=3), "fp8 output")])
 def test_decode_attention_refuses(change, match):
     args = dict(ATTN, **ATTN_OUT)
