@@ -398,7 +398,8 @@ int qb_decode_attention_workspace(int64_t* bytes);
  * out and q_out both: out: bf16, rows out_ld apart (a multiple of 4);
  * q_out: fp8 [rows, n_q * 128] with scale_out f32 [n_q, scale_ld], the bf16
  * output quantised per head as qb_tree_attention's (head_dim 128 only);
- * lse_out: f32 [rows, n_q]. n_q a multiple of n_kv; head_dim 64 or 128;
+ * lse_out: f32 [rows, n_q]. n_q a multiple of n_kv, at most 4096; head_dim
+ * 64 or 128; table_width * page_tokens at most 2^30;
  * page_tokens a power of two from 8 to 1024; rows <= 65,535; q and the pools
  * 16-byte aligned. A page or a used[r] out of range sets
  * QB_STATUS_BAD_INDEX; such keys are left out.

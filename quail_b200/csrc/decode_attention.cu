@@ -38,12 +38,16 @@ namespace {
 
 using namespace qb;
 
-constexpr int WARPS = 8;      // of one block; they take a head's key steps in turn
-constexpr int HEADS = 8;      // query heads of a block: the MMA's N
-constexpr int STEP = 16;      // keys of a warp's step, and of a unit of work
-constexpr int BLOCKS_PER_SM = 2;
-constexpr int MIN_UNITS = WARPS;        // a block's least part of an item: a step a warp
-constexpr int WHOLE_UNITS = 2 * WARPS;  // items up to this long are not cut
+constexpr int HEADS = 8;      // query heads of an item: the MMA's N
+constexpr int UNIT_SHIFT = 4; // a unit of work: 16 keys
+constexpr int MIN_UNITS = 8;          // a block's least part of an item that is cut
+constexpr int WHOLE_UNITS = 16;       // items up to this long are not cut
+
+// Warps of a block, one block an SM.
+template <bool FP8>
+constexpr int warps() {
+    return FP8 ? 8 : 12;
+}
 constexpr float LN2 = 0.693147180559945309f;
 constexpr float LOG2E = 1.44269504088896341f;
 
@@ -60,6 +64,7 @@ struct Params {
     const bf16* q;
     int64_t q_ld;
     int rows;
+    int unit_shift;                   // log2 of the keys of a unit of work
     int n_q, n_kv, group;             // group = n_q / n_kv
     int tiles;                        // ceil(group / HEADS) blocks share a KV head
     const void* k;
@@ -93,16 +98,32 @@ __device__ __forceinline__ int row_keys(const Params& p, int r, bool flag) {
     return n < 0 ? 0 : most;
 }
 
-// Where a block's range ends: the item there, as its place in the row order.
-struct Cut {
-    int64_t at;       // unit, over all items
-    int64_t before;   // units of the rows before `row`, one head
-    int row;
+__device__ __forceinline__ int units_of(const Params& p, int keys) {
+    return (int)(((int64_t)keys + (1 << p.unit_shift) - 1) >> p.unit_shift);
+}
+
+// A place in the line of all items' units (which holds under 2^31 of them, by
+// the choice of the unit).
+struct Place {
+    int at;       // the unit
+    int row;      // its row
+    int before;   // units of one head of the rows before it
 };
 
-// The cut x of [0, total) moved off short items and slivers: within the item
-// [s, s + n)
-__device__ __forceinline__ int64_t settle(int64_t x, int64_t s, int n) {
+// Range i of `n` that `total` is cut into begins at i * base + min(i, rest).
+struct Cuts {
+    int base, rest;
+    __device__ __forceinline__ Cuts(int total, int n) : base(total / n) { rest = total - base * n; }
+    __device__ __forceinline__ int at(int i) const { return i * base + min(i, rest); }
+    // the first range that begins at x or later
+    __device__ __forceinline__ int from(int x) const {
+        const int wide = rest * (base + 1);
+        return x <= wide ? (x + base) / (base + 1) : rest + (x - wide + base - 1) / base;
+    }
+};
+
+// The cut x moved off short items and slivers, within the item [s, s + n)
+__device__ __forceinline__ int settle(int x, int s, int n) {
     if (n <= WHOLE_UNITS || x - s < MIN_UNITS) return s;
     return s + n - x < MIN_UNITS ? s + n : x;
 }
@@ -174,7 +195,7 @@ template <int D>
 struct alignas(16) Slot {
     float o[HEADS][D + 4];
     float m[HEADS], l[HEADS], mv[HEADS];
-    int64_t start;       // the item's first unit, over all items; -1: no part
+    int start;           // the item's first unit, over all items; -1: no part
     int n, row, item;    // its units, row and place in the row
     int whole;           // 2: starts the item, 1: ends it
 };
@@ -193,7 +214,6 @@ __device__ __forceinline__ void attend(const Params& p, Slot<D>& slot, int row, 
     constexpr int VC = FP8 ? 1 : D / 64;         // chunks of a V row a lane
     constexpr int MT = D / 16;                   // 16-row tiles of O^T
     const int g = lane >> 2, t = lane & 3;
-    const int page = 1 << p.page_shift;
     const int32_t* table = p.table + row * p.table_ld;
 
     // Q as the B fragments of S^T: this lane's columns of head g
@@ -264,126 +284,170 @@ __device__ __forceinline__ void attend(const Params& p, Slot<D>& slot, int row, 
 #pragma unroll
         for (int j = 0; j < 4; ++j) o[i][j] = 0.0f;
 
+    // A step: 16 keys of 128 bf16, else 32. The pipeline: while a step is
+    // computed, the next one's K (as soon as S has consumed the registers), V
+    // (after the second product) and, one further, the page ids are on their
+    // way.
+    constexpr int UNITS = FP8 || D == 64 ? 2 : 1;
     const int64_t row_bytes = (int64_t)p.n_kv * D * ELEM;
-    const char* k_base = (const char*)p.k + (int64_t)kvh * D * ELEM;
-    const char* v_base = (const char*)p.v + (int64_t)kvh * D * ELEM;
+    const int64_t page_bytes = row_bytes << p.page_shift;
+    const char* k_lane = (const char*)p.k + (int64_t)kvh * D * ELEM + g * row_bytes + t * 16;
+    const char* v_lane = (const char*)p.v + (int64_t)kvh * D * ELEM + 2 * t * row_bytes +
+                         g * (FP8 && D == 64 ? 8 : 16);
+    const int n_pages = (int)min(p.n_pages, (int64_t)0x7fffffff);
+    const int mask = (1 << p.page_shift) - 1;
 
-    for (; key0 < end; key0 += STEP) {
-        // a page holds a multiple of 8 tokens, so each half step is in one page
-        int64_t half_row[2];
-        bool half_ok[2];
+    uint4 kr[UNITS][2][KC], vr[UNITS][4][VC];
+    uint32_t kb[UNITS][2], vb[UNITS][2];   // 8 bit: exponent bytes of keys g and g + 8
+    int ids[UNITS][2];                     // pages of the half steps, -1: none
+    // a page holds a multiple of 8 tokens, so each half step is in one page
+    auto find = [&](int key0) {
 #pragma unroll
-        for (int h = 0; h < 2; ++h) {
-            const int key = key0 + 8 * h;
-            const int id = key < end ? table[key >> p.page_shift] : 0;
-            half_ok[h] = key < end && id >= 0 && id < p.n_pages;
-            if (key < end && !half_ok[h] && lane == 0) atomicOr(p.status, STATUS_BAD_INDEX);
-            half_row[h] = ((int64_t)(half_ok[h] ? id : 0) << p.page_shift) + (key & (page - 1));
-        }
-        // ---- K: rows g and g + 8 of the step
-        uint4 kr[2][KC];
-        float kx[2] = {1.0f, 1.0f};
-        bool k_ok[2];
+        for (int u = 0; u < UNITS; ++u)
 #pragma unroll
-        for (int h = 0; h < 2; ++h) {
-            k_ok[h] = half_ok[h] && key0 + 8 * h + g < end;
-            const int64_t at = half_row[h] + g;
-#pragma unroll
-            for (int c = 0; c < KC; ++c)
-                kr[h][c] = k_ok[h] ? load16(k_base + at * row_bytes + (t + 4 * c) * 16)
-                                   : make_uint4(0, 0, 0, 0);
-            if (FP8 && k_ok[h]) kx[h] = e8m0_float(p.k_scale[at * p.n_kv + kvh]);
-        }
-        // ---- V: rows 2t, 2t + 1 of each half; codes of keys past the end
-        // are zeros, for 0 * NaN is NaN
-        uint4 vr[4][VC];
-        float vb[2] = {0.0f, 0.0f};   // exponents of keys g and g + 8
-#pragma unroll
-        for (int r = 0; r < 4; ++r) {
-            const int h = r >> 1, off = 2 * t + (r & 1);
-            const bool ok = half_ok[h] && key0 + 8 * h + off < end;
-            const int64_t at = half_row[h] + off;
-#pragma unroll
-            for (int c = 0; c < VC; ++c) {
-                vr[r][c] = make_uint4(0, 0, 0, 0);
-                if (FP8 && D == 64) {
-                    if (ok) {
-                        const uint2 w = load8(v_base + at * row_bytes + g * 8);
-                        vr[r][c].x = w.x;
-                        vr[r][c].y = w.y;
-                    }
-                } else if (ok) {
-                    vr[r][c] = load16(v_base + at * row_bytes + (g + 8 * c) * 16);
-                }
+            for (int h = 0; h < 2; ++h) {
+                const int key = key0 + 16 * u + 8 * h;
+                ids[u][h] = key < end ? __ldg(table + (key >> p.page_shift)) : -1;
             }
-        }
-        if (FP8) {
+    };
+    auto check = [&](int key0) {
+#pragma unroll
+        for (int u = 0; u < UNITS; ++u)
 #pragma unroll
             for (int h = 0; h < 2; ++h)
-                if (k_ok[h]) {
-                    const uint32_t b = p.v_scale[(half_row[h] + g) * p.n_kv + kvh];
-                    vb[h] = b == 255u ? __uint_as_float(0x7FFFFFFFu) : (float)((int)b - 127);
+                if ((uint32_t)ids[u][h] >= (uint32_t)n_pages) {
+                    if (key0 + 16 * u + 8 * h < end && lane == 0)
+                        atomicOr(p.status, STATUS_BAD_INDEX);
+                    ids[u][h] = -1;
                 }
-        }
+    };
+    // bit 2u + h: key g of that half step is one
+    auto load_k = [&](int key0) {
+        uint32_t ok = 0;
+#pragma unroll
+        for (int u = 0; u < UNITS; ++u)
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+                const int key = key0 + 16 * u + 8 * h;
+                const bool in = ids[u][h] >= 0 && key + g < end;
+                const char* at = k_lane + ids[u][h] * page_bytes + (key & mask) * row_bytes;
+                ok |= in ? 1u << (2 * u + h) : 0u;
+#pragma unroll
+                for (int c = 0; c < KC; ++c)
+                    kr[u][h][c] = in ? load16(at + 64 * c) : make_uint4(0, 0, 0, 0);
+                if (FP8) {
+                    const int64_t row =
+                        ((int64_t)ids[u][h] << p.page_shift) + (key & mask) + g;
+                    kb[u][h] = in ? p.k_scale[row * p.n_kv + kvh] : 127u;
+                    vb[u][h] = in ? p.v_scale[row * p.n_kv + kvh] : 127u;
+                }
+            }
+        return ok;
+    };
+    // V: rows 2t, 2t + 1 of each half; keys past the end are zeros, for
+    // 0 * NaN is NaN
+    auto load_v = [&](int key0) {
+#pragma unroll
+        for (int u = 0; u < UNITS; ++u)
+#pragma unroll
+            for (int r = 0; r < 4; ++r) {
+                const int h = r >> 1, key = key0 + 16 * u + 8 * h;
+                const bool in = ids[u][h] >= 0 && key + 2 * t + (r & 1) < end;
+                const char* at = v_lane + ids[u][h] * page_bytes +
+                                 ((key & mask) + (r & 1)) * row_bytes;
+#pragma unroll
+                for (int c = 0; c < VC; ++c) {
+                    vr[u][r][c] = make_uint4(0, 0, 0, 0);
+                    if (FP8 && D == 64) {
+                        if (in) {
+                            const uint2 w = load8(at);
+                            vr[u][r][c].x = w.x;
+                            vr[u][r][c].y = w.y;
+                        }
+                    } else if (in) {
+                        vr[u][r][c] = load16(at + 128 * c);
+                    }
+                }
+            }
+    };
 
+    find(key0);
+    check(key0);
+    uint32_t k_ok = load_k(key0);
+    load_v(key0);
+    find(key0 + 16 * UNITS);
+    for (; key0 < end; key0 += 16 * UNITS) {
         // ---- S^T: keys g and g + 8, heads 2t and 2t + 1
-        float s[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+        float s[UNITS][4];
 #pragma unroll
-        for (int c = 0; c < KC; ++c) {
-            const uint32_t w0[4] = {kr[0][c].x, kr[0][c].y, kr[0][c].z, kr[0][c].w};
-            const uint32_t w1[4] = {kr[1][c].x, kr[1][c].y, kr[1][c].z, kr[1][c].w};
-            if (FP8) {
+        for (int u = 0; u < UNITS; ++u) {
 #pragma unroll
-                for (int w = 0; w < 4; ++w)
-                    mma16816<true>(s, e4m3x2_f16x2(w0[w]), e4m3x2_f16x2(w1[w]),
-                                   e4m3x2_f16x2(w0[w] >> 16), e4m3x2_f16x2(w1[w] >> 16),
-                                   qf[8 * c + 2 * w], qf[8 * c + 2 * w + 1]);
-            } else {
+            for (int i = 0; i < 4; ++i) s[u][i] = 0.0f;
 #pragma unroll
-                for (int w = 0; w < 2; ++w)
-                    mma16816<false>(s, w0[2 * w], w1[2 * w], w0[2 * w + 1], w1[2 * w + 1],
-                                    qf[4 * c + 2 * w], qf[4 * c + 2 * w + 1]);
+            for (int c = 0; c < KC; ++c) {
+                const uint32_t w0[4] = {kr[u][0][c].x, kr[u][0][c].y, kr[u][0][c].z,
+                                        kr[u][0][c].w};
+                const uint32_t w1[4] = {kr[u][1][c].x, kr[u][1][c].y, kr[u][1][c].z,
+                                        kr[u][1][c].w};
+                if (FP8) {
+#pragma unroll
+                    for (int w = 0; w < 4; ++w)
+                        mma16816<true>(s[u], e4m3x2_f16x2(w0[w]), e4m3x2_f16x2(w1[w]),
+                                       e4m3x2_f16x2(w0[w] >> 16), e4m3x2_f16x2(w1[w] >> 16),
+                                       qf[8 * c + 2 * w], qf[8 * c + 2 * w + 1]);
+                } else {
+#pragma unroll
+                    for (int w = 0; w < 2; ++w)
+                        mma16816<false>(s[u], w0[2 * w], w1[2 * w], w0[2 * w + 1], w1[2 * w + 1],
+                                        qf[4 * c + 2 * w], qf[4 * c + 2 * w + 1]);
+                }
             }
         }
-        float x[4], y[4];   // index 2 * half + head; y: the exponent with the value's scale
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            x[i] = s[i] * x_scale[i & 1];
-            if (FP8) x[i] *= kx[i >> 1];
-            if (!k_ok[i >> 1]) x[i] = NEG_INF;
-            y[i] = FP8 ? x[i] + vb[i >> 1] : x[i];
-        }
+        float x[UNITS][4], y[UNITS][4];   // [2 * half + head]; y: x and the value's exponent
         bool raise = false;
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            raise |= x[i] > top[i & 1] + SLACK;
-            if (FP8) raise |= y[i] > top_v[i & 1] + SLACK;
-        }
+        for (int u = 0; u < UNITS; ++u)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                float v = s[u][i] * x_scale[i & 1];
+                if (FP8) v *= e8m0_float(kb[u][i >> 1]);
+                if (!(k_ok >> (2 * u + (i >> 1)) & 1)) v = NEG_INF;
+                x[u][i] = y[u][i] = v;
+                raise |= v > top[i & 1] + SLACK;
+                if (FP8) {
+                    const uint32_t b = vb[u][i >> 1];
+                    y[u][i] += b == 255u ? __uint_as_float(0x7FFFFFFFu) : (float)((int)b - 127);
+                    raise |= y[u][i] > top_v[i & 1] + SLACK;
+                }
+            }
+        check(key0 + 16 * UNITS);
+        k_ok = load_k(key0 + 16 * UNITS);
         if (__any_sync(0xffffffffu, raise)) {
 #pragma unroll
             for (int n = 0; n < 2; ++n) {
-                float a = fmaxf(x[n], x[2 + n]), b = fmaxf(y[n], y[2 + n]);
+                float a = top[n], b = top_v[n];
+#pragma unroll
+                for (int u = 0; u < UNITS; ++u) {
+                    a = fmax3(a, x[u][n], x[u][2 + n]);
+                    b = fmax3(b, y[u][n], y[u][2 + n]);
+                }
 #pragma unroll
                 for (int off = 4; off < 32; off <<= 1) {
                     a = fmaxf(a, __shfl_xor_sync(0xffffffffu, a, off));
                     if (FP8) b = fmaxf(b, __shfl_xor_sync(0xffffffffu, b, off));
                 }
-                a = fmaxf(a, top[n]);
-                const float old = ref[n];
                 float down = 0.0f;
                 if (a > NEG_INF) {
+                    if (top[n] > NEG_INF) down = exp2_approx(ref[n] - a);
                     ref[n] = a;
-                    if (top[n] > NEG_INF) down = exp2_approx(old - a);
                 }
                 top[n] = a;
                 sum[n] *= down;
                 if (FP8) {
-                    b = fmaxf(b, top_v[n]);
-                    const float old_v = ref_v[n];
                     down = 0.0f;
                     if (b > NEG_INF) {
+                        if (top_v[n] > NEG_INF) down = exp2_approx(ref_v[n] - b);
                         ref_v[n] = b;
-                        if (top_v[n] > NEG_INF) down = exp2_approx(old_v - b);
                     }
                     top_v[n] = b;
                 }
@@ -394,56 +458,65 @@ __device__ __forceinline__ void attend(const Params& p, Slot<D>& slot, int row, 
                 }
             }
         }
-        float w[4];
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            const float e = exp2_approx(x[i] - ref[i & 1]);
-            sum[i & 1] += e;
-            w[i] = FP8 ? exp2_approx(y[i] - ref_v[i & 1] + LIFT) : e;
-        }
         // ---- O^T += V^T P^T: the weights as B fragments, by a transpose.
         // bf16 keeps 8 bits of a weight, so what it drops goes through a second
         // product; f16 keeps 11 and needs none.
-        uint32_t hi[2], lo[2];
 #pragma unroll
-        for (int h = 0; h < 2; ++h) {
-            if (FP8) {
-                hi[h] = transpose8(half2_bits(w[2 * h], w[2 * h + 1]));
-            } else {
-                const uint32_t b = bf16x2_bits(w[2 * h], w[2 * h + 1]);
-                const float2 f = bf16x2_float2(b);
-                hi[h] = transpose8(b);
-                lo[h] = transpose8(bf16x2_bits(w[2 * h] - f.x, w[2 * h + 1] - f.y));
+        for (int u = 0; u < UNITS; ++u) {
+            float w[4];
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const float e = exp2_approx(x[u][i] - ref[i & 1]);
+                sum[i & 1] += e;
+                w[i] = FP8 ? exp2_approx(y[u][i] - ref_v[i & 1] + LIFT) : e;
             }
-        }
+            uint32_t hi[2], lo[2];
 #pragma unroll
-        for (int c = 0; c < VC; ++c) {
-            const uint32_t v0[4] = {vr[0][c].x, vr[0][c].y, vr[0][c].z, vr[0][c].w};
-            const uint32_t v1[4] = {vr[1][c].x, vr[1][c].y, vr[1][c].z, vr[1][c].w};
-            const uint32_t v2[4] = {vr[2][c].x, vr[2][c].y, vr[2][c].z, vr[2][c].w};
-            const uint32_t v3[4] = {vr[3][c].x, vr[3][c].y, vr[3][c].z, vr[3][c].w};
-#pragma unroll
-            for (int i = 0; i < (FP8 && D == 64 ? 2 : 4); ++i) {
+            for (int h = 0; h < 2; ++h) {
                 if (FP8) {
-                    // four columns of keys 2t, 2t + 1 (a) and 2t + 8, 2t + 9 (b)
-                    const uint32_t a01 = __byte_perm(v0[i], v1[i], 0x5140);
-                    const uint32_t a23 = __byte_perm(v0[i], v1[i], 0x7362);
-                    const uint32_t b01 = __byte_perm(v2[i], v3[i], 0x5140);
-                    const uint32_t b23 = __byte_perm(v2[i], v3[i], 0x7362);
-                    mma16816<true>(o[2 * i], e4m3x2_f16x2(a01), e4m3x2_f16x2(a01 >> 16),
-                                   e4m3x2_f16x2(b01), e4m3x2_f16x2(b01 >> 16), hi[0], hi[1]);
-                    mma16816<true>(o[2 * i + 1], e4m3x2_f16x2(a23), e4m3x2_f16x2(a23 >> 16),
-                                   e4m3x2_f16x2(b23), e4m3x2_f16x2(b23 >> 16), hi[0], hi[1]);
+                    hi[h] = transpose8(half2_bits(w[2 * h], w[2 * h + 1]));
                 } else {
-                    const uint32_t a0 = __byte_perm(v0[i], v1[i], 0x5410);
-                    const uint32_t a1 = __byte_perm(v0[i], v1[i], 0x7632);
-                    const uint32_t a2 = __byte_perm(v2[i], v3[i], 0x5410);
-                    const uint32_t a3 = __byte_perm(v2[i], v3[i], 0x7632);
-                    mma16816<false>(o[4 * c + i], a0, a1, a2, a3, hi[0], hi[1]);
-                    mma16816<false>(o[4 * c + i], a0, a1, a2, a3, lo[0], lo[1]);
+                    const uint32_t b = bf16x2_bits(w[2 * h], w[2 * h + 1]);
+                    const float2 f = bf16x2_float2(b);
+                    hi[h] = transpose8(b);
+                    lo[h] = transpose8(bf16x2_bits(w[2 * h] - f.x, w[2 * h + 1] - f.y));
+                }
+            }
+#pragma unroll
+            for (int c = 0; c < VC; ++c) {
+                uint32_t v[4][4];
+#pragma unroll
+                for (int r = 0; r < 4; ++r) {
+                    v[r][0] = vr[u][r][c].x;
+                    v[r][1] = vr[u][r][c].y;
+                    v[r][2] = vr[u][r][c].z;
+                    v[r][3] = vr[u][r][c].w;
+                }
+#pragma unroll
+                for (int i = 0; i < (FP8 && D == 64 ? 2 : 4); ++i) {
+                    if (FP8) {
+                        // four columns of keys 2t, 2t + 1 (a) and 2t + 8, 2t + 9 (b)
+                        const uint32_t a01 = __byte_perm(v[0][i], v[1][i], 0x5140);
+                        const uint32_t a23 = __byte_perm(v[0][i], v[1][i], 0x7362);
+                        const uint32_t b01 = __byte_perm(v[2][i], v[3][i], 0x5140);
+                        const uint32_t b23 = __byte_perm(v[2][i], v[3][i], 0x7362);
+                        mma16816<true>(o[2 * i], e4m3x2_f16x2(a01), e4m3x2_f16x2(a01 >> 16),
+                                       e4m3x2_f16x2(b01), e4m3x2_f16x2(b01 >> 16), hi[0], hi[1]);
+                        mma16816<true>(o[2 * i + 1], e4m3x2_f16x2(a23), e4m3x2_f16x2(a23 >> 16),
+                                       e4m3x2_f16x2(b23), e4m3x2_f16x2(b23 >> 16), hi[0], hi[1]);
+                    } else {
+                        const uint32_t a0 = __byte_perm(v[0][i], v[1][i], 0x5410);
+                        const uint32_t a1 = __byte_perm(v[0][i], v[1][i], 0x7632);
+                        const uint32_t a2 = __byte_perm(v[2][i], v[3][i], 0x5410);
+                        const uint32_t a3 = __byte_perm(v[2][i], v[3][i], 0x7632);
+                        mma16816<false>(o[4 * c + i], a0, a1, a2, a3, hi[0], hi[1]);
+                        mma16816<false>(o[4 * c + i], a0, a1, a2, a3, lo[0], lo[1]);
+                    }
                 }
             }
         }
+        load_v(key0 + 16 * UNITS);
+        find(key0 + 32 * UNITS);
     }
 
     // ---- the warp's sums, and its state to shared memory
@@ -480,7 +553,7 @@ struct Joined {
     }
     // x against the exponent `from`, brought to `to`; nothing has `from` -inf
     static __device__ __forceinline__ float factor(float from, float to) {
-        return from > __uint_as_float(0xFF800000u) ? exp2f(from - to) : 0.0f;
+        return from > __uint_as_float(0xFF800000u) ? exp2_approx(from - to) : 0.0f;
     }
     __device__ __forceinline__ void add(float mi, float li, float mvi, const float4& part) {
         const float top = fmaxf(m, mi);
@@ -510,9 +583,10 @@ __device__ __forceinline__ void finish(const Params& p, const Joined<FP8>& j, in
     const float NEG_INF = __uint_as_float(0xFF800000u);
     float r[4] = {0.0f, 0.0f, 0.0f, 0.0f};
     if (j.l != 0.0f) {   // a NaN stays one
-        const float f = FP8 && j.mv > NEG_INF ? exp2f(j.mv - j.m - LIFT) : 1.0f;
+        float f = 1.0f / j.l;
+        if (FP8 && j.mv > NEG_INF) f *= exp2f(j.mv - j.m - LIFT);
 #pragma unroll
-        for (int i = 0; i < 4; ++i) r[i] = j.acc[i] / j.l * f;
+        for (int i = 0; i < 4; ++i) r[i] = j.acc[i] * f;
     }
     if (live) {
         if (p.lse && d4 == 0)
@@ -546,181 +620,175 @@ __device__ __forceinline__ void finish(const Params& p, const Joined<FP8>& j, in
     }
 }
 
-__device__ __forceinline__ int64_t ceil_div(int64_t a, int64_t b) { return (a + b - 1) / b; }
-
-// The row at or after `row` (`before`: one head's units of the rows before it)
-// that holds unit `at`, and its units n. One warp.
-__device__ __forceinline__ void find_row(const Params& p, int64_t at, int per_row, int lane,
-                                         int& row, int64_t& before, int& n) {
-    for (;;) {
-        const int r = row + lane;
-        const int mine = r < p.rows ? (row_keys(p, r, false) + STEP - 1) / STEP : 0;
-        int64_t upto = mine;
-#pragma unroll
-        for (int o = 1; o < 32; o <<= 1) {
-            const int64_t u = __shfl_up_sync(0xffffffffu, upto, o);
-            if (lane >= o) upto += u;
-        }
-        const uint32_t past = __ballot_sync(0xffffffffu, at < (before + upto) * per_row);
-        const int hit = past ? __ffs(past) - 1 : 31;
-        const int64_t through = __shfl_sync(0xffffffffu, upto, hit);
-        n = __shfl_sync(0xffffffffu, mine, hit);
-        row += hit;
-        before += through - n;
-        if (past || row + 1 >= p.rows) return;
-        before += n;
-        row += 1;
-    }
-}
-
 template <int D, bool FP8>
-__global__ void __launch_bounds__(WARPS * 32, BLOCKS_PER_SM)
+__global__ void __launch_bounds__(warps<FP8>() * 32, 1)
 decode_attention_kernel(const Params p) {
+    constexpr int WARPS = warps<FP8>();
     constexpr int THREADS = WARPS * 32;
     constexpr int QUADS = D / 4;   // threads of a head in the join
     extern __shared__ __align__(16) char smem[];
     Slot<D>* slots = reinterpret_cast<Slot<D>*>(smem);   // [WARPS][2]: begun before, begun here
-    __shared__ int64_t s_scan[WARPS], s_items[WARPS];
-    __shared__ Cut s_cut[2];
+    __shared__ int s_scan[WARPS], s_full[WARPS];
+    __shared__ Place s_cut[2], s_start[WARPS];
     __shared__ uint32_t s_last;
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     const int per_row = p.n_kv * p.tiles;   // items of a row
 
-    // ---- this block's range: a scan over the rows' units
+    // ---- a scan over the rows' units: this thread's rows hold [from, to)
     const int chunk = (p.rows + THREADS - 1) / THREADS;
     const int r0 = min(tid * chunk, p.rows), r1 = min(r0 + chunk, p.rows);
-    int64_t mine = 0;
-    int full = 0;   // rows that hold keys
+    int mine = 0, full = 0;
     for (int r = r0; r < r1; ++r) {
-        const int n = (row_keys(p, r, blockIdx.x == 0) + STEP - 1) / STEP;
+        const int n = units_of(p, row_keys(p, r, blockIdx.x == 0));
         mine += n;
         full += n > 0;
     }
-    int64_t upto = mine;
+    int upto = mine;
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
-        const int64_t u = __shfl_up_sync(0xffffffffu, upto, o);
+        const int u = __shfl_up_sync(0xffffffffu, upto, o);
         if (lane >= o) upto += u;
     }
     full = __reduce_add_sync(0xffffffffu, full);
     if (lane == 31) {
         s_scan[warp] = upto;
-        s_items[warp] = full;
+        s_full[warp] = full;
     }
+    if (lane < 2) slots[2 * warp + lane].start = -1;
     __syncthreads();
-    int64_t units = 0, items = 0;
+    int units = 0;
+    full = 0;
 #pragma unroll
     for (int w = 0; w < WARPS; ++w) {
         if (w < warp) upto += s_scan[w];
         units += s_scan[w];
-        items += s_items[w];
+        full += s_full[w];
     }
-    const int64_t total = units * per_row;
-    items *= per_row;
+    const int first_unit = upto - mine;   // of one head
+    const int from = first_unit * per_row, to = upto * per_row;
+    const int total = units * per_row;
+    // rows without keys
+    if (full < p.rows)
+        for (int r = blockIdx.x; r < p.rows; r += gridDim.x) {
+            if (row_keys(p, r, false) != 0) continue;
+            const Joined<FP8> none;
+            for (int i = tid; i < p.n_q * QUADS; i += THREADS)
+                finish<D, FP8>(p, none, r, i / QUADS, true, i % QUADS * 4);
+        }
     // a block an item where the items are short, and no block under MIN_UNITS
     // of a long one
-    const int64_t blocks = min((int64_t)gridDim.x, max(items, total / MIN_UNITS));
-    if ((int64_t)blockIdx.x < blocks) {
-#pragma unroll
-        for (int c = 0; c < 2; ++c) {
-            const int64_t g = (int64_t)blockIdx.x + c;
-            const int64_t x = g == blocks ? total : total * g / blocks;
-            if (g == blocks) {
-                if (tid == 0) s_cut[c].at = total;
-            } else if (x >= (upto - mine) * per_row && x < upto * per_row) {
-                int64_t before = upto - mine;
-                int r = r0, n = 0;
-                for (; r < r1; ++r) {
-                    n = (row_keys(p, r, false) + STEP - 1) / STEP;
-                    if (x < (before + n) * per_row) break;
-                    before += n;
-                }
-                const int64_t s = before * per_row + (x - before * per_row) / n * n;
-                s_cut[c].at = settle(x, s, n);
-                s_cut[c].before = before;
-                s_cut[c].row = r;
-            }
-        }
-    }
-    // rows without keys
-    for (int r = blockIdx.x; r < p.rows; r += gridDim.x) {
-        if (row_keys(p, r, false) != 0) continue;
-        const Joined<FP8> none;
-        for (int i = tid; i < p.n_q * QUADS; i += THREADS)
-            finish<D, FP8>(p, none, r, i / QUADS, true, i % QUADS * 4);
-    }
-    if ((int64_t)blockIdx.x >= blocks) return;
-    __syncthreads();
-    const int64_t lo = s_cut[0].at, hi = s_cut[1].at;
+    const int blocks = min((int)gridDim.x, max(full * per_row, total / MIN_UNITS));
+    if ((int)blockIdx.x >= blocks) return;
 
-    // ---- this warp's range
-    if (lane < 2) slots[2 * warp + lane].start = -1;
-    __syncwarp();
-    int64_t at = lo + (hi - lo) * warp / WARPS;
-    const int64_t end = lo + (hi - lo) * (warp + 1) / WARPS;
-    int row = s_cut[0].row, n = 0;
-    int64_t before = s_cut[0].before;
-    while (at < end) {
-        if (at >= (before + n) * per_row || n == 0) find_row(p, at, per_row, lane, row, before, n);
-        const int item = (int)(at - before * per_row) / n;
-        const int64_t s = before * per_row + (int64_t)item * n;
-        const int64_t stop = min(end, s + n);
-        const int kvh = item / p.tiles, tile = item % p.tiles;
-        const int head0 = kvh * p.group + tile * HEADS;
-        const int heads = min(HEADS, p.group - tile * HEADS);
-        const int whole = 2 * (at == s) + (stop == s + n);
-        Slot<D>& slot = slots[2 * warp + (at == s)];
-        attend<D, FP8>(p, slot, row, kvh, head0, heads, (int)(at - s) * STEP,
-                       min(row_keys(p, row, false), (int)(stop - s) * STEP), lane);
-        __syncwarp();
-        if (whole == 3) {
-            for (int i = lane; i < HEADS * QUADS; i += 32) {
-                const int head = i / QUADS, d4 = i % QUADS * 4;
-                if (D == 128 && head >= heads) break;   // D = 64: two heads at a time
-                Joined<FP8> j;
-                j.add(slot.m[head], slot.l[head], slot.mv[head],
-                      *reinterpret_cast<const float4*>(&slot.o[head][d4]));
-                finish<D, FP8>(p, j, row, head0 + head, head < heads, d4);
-            }
-        } else if (lane == 0) {
-            slot.start = s;
-            slot.n = n;
-            slot.row = row;
-            slot.item = item;
-            slot.whole = whole;
+    // ---- this block's range, and its warps'
+    const Cuts cuts(total, blocks);
+    // the place of unit x, which is one of this thread's; its item's units in n
+    auto place = [&](int x, int& n) {
+        Place at = {x, r0, first_unit};
+        for (; at.row < r1; ++at.row) {
+            n = units_of(p, row_keys(p, at.row, false));
+            if (x < (at.before + n) * per_row) break;
+            at.before += n;
         }
-        __syncwarp();
-        at = stop;
+        return at;
+    };
+#pragma unroll
+    for (int c = 0; c < 2; ++c) {
+        const int i = blockIdx.x + c;
+        const int x = cuts.at(i);
+        if (x >= from && x < to) {
+            int n;
+            Place at = place(x, n);
+            const int s = at.before * per_row;
+            at.at = settle(x, s + (x - s) / n * n, n);
+            s_cut[c] = at;
+        }
+        if (i == blocks && tid == 0) s_cut[c].at = total;
+    }
+    __syncthreads();
+    const int lo = s_cut[0].at, hi = s_cut[1].at;
+    if (lo == hi) return;   // an item that a neighbour has whole
+    const Cuts shares(hi - lo, WARPS);
+    if (from < hi && to > lo) {
+#pragma unroll
+        for (int w = 0; w < WARPS; ++w) {
+            const int x = lo + shares.at(w);
+            int n;
+            if (x >= from && x < to) s_start[w] = place(x, n);
+        }
+    }
+    __syncthreads();
+
+    // ---- this warp's range, an item after another
+    int at = lo + shares.at(warp);
+    const int end = lo + shares.at(warp + 1);
+    if (at < end) {
+        int row = s_start[warp].row, before = s_start[warp].before;
+        int keys = row_keys(p, row, false), n = units_of(p, keys);
+        for (;;) {
+            const int item = (at - before * per_row) / n;
+            const int s = before * per_row + item * n;
+            const int stop = min(end, s + n);
+            const int kvh = item / p.tiles, tile = item % p.tiles;
+            const int head0 = kvh * p.group + tile * HEADS;
+            const int heads = min(HEADS, p.group - tile * HEADS);
+            const int whole = 2 * (at == s) + (stop == s + n);
+            Slot<D>& slot = slots[2 * warp + (at == s)];
+            attend<D, FP8>(p, slot, row, kvh, head0, heads, (at - s) << p.unit_shift,
+                           (int)min((int64_t)keys, (int64_t)(stop - s) << p.unit_shift), lane);
+            __syncwarp();
+            if (whole == 3) {
+                for (int i = lane; i < HEADS * QUADS; i += 32) {
+                    const int head = i / QUADS, d4 = i % QUADS * 4;
+                    if (D == 128 && head >= heads) break;   // D = 64: two heads at a time
+                    Joined<FP8> j;
+                    j.add(slot.m[head], slot.l[head], slot.mv[head],
+                          *reinterpret_cast<const float4*>(&slot.o[head][d4]));
+                    finish<D, FP8>(p, j, row, head0 + head, head < heads, d4);
+                }
+            } else if (lane == 0) {
+                slot.start = s;
+                slot.n = n;
+                slot.row = row;
+                slot.item = item;
+                slot.whole = whole;
+            }
+            __syncwarp();
+            at = stop;
+            if (at >= end) break;
+            while (at >= (before + n) * per_row) {
+                before += n;
+                ++row;
+                keys = row_keys(p, row, false);
+                n = units_of(p, keys);
+            }
+        }
     }
     __syncthreads();
 
     // ---- the parts that warps share, in order
     const int my_head = tid / QUADS, d4 = tid % QUADS * 4;
-    const bool have = my_head < HEADS;   // D = 64 leaves half of the threads over
-    for (int i = 0; i < 2 * WARPS;) {
-        const int64_t s = slots[i].start;
-        if (s < 0) {
-            ++i;
-            continue;
-        }
-        const int row = slots[i].row, item = slots[i].item;
-        const int64_t n = slots[i].n;
+    const bool have = my_head < HEADS;   // the threads past the heads' columns help nothing
+    const int start = lane < 2 * WARPS ? slots[lane].start : -1;
+    uint32_t left = __ballot_sync(0xffffffffu, start >= 0);
+    while (left) {
+        const int i = __ffs(left) - 1;
+        const int s = __shfl_sync(0xffffffffu, start, i);
+        uint32_t chain = __ballot_sync(0xffffffffu, start == s);
+        left &= ~chain;
+        const int row = slots[i].row, item = slots[i].item, n = slots[i].n;
         const int kvh = item / p.tiles, tile = item % p.tiles;
         const int head0 = kvh * p.group + tile * HEADS;
         const int heads = min(HEADS, p.group - tile * HEADS);
         const bool begins = slots[i].whole & 2;
-        bool ends = false;
+        bool whole = begins && (slots[31 - __clz(chain)].whole & 1);
         Joined<FP8> j;
-        for (; i < 2 * WARPS; ++i) {
-            const Slot<D>& slot = slots[i];
-            if (slot.start < 0) continue;
-            if (slot.start != s) break;
-            ends = slot.whole & 1;
-            if (have)
+        if (have)
+            for (; chain; chain &= chain - 1) {
+                const Slot<D>& slot = slots[__ffs(chain) - 1];
                 j.add(slot.m[my_head], slot.l[my_head], slot.mv[my_head],
                       *reinterpret_cast<const float4*>(&slot.o[my_head][d4]));
-        }
-        bool whole = begins && ends;
+            }
         if (!whole) {
             Part<D>* parts = (Part<D>*)p.parts;
             Part<D>& part = parts[2 * blockIdx.x + begins];
@@ -734,8 +802,8 @@ decode_attention_kernel(const Params p) {
                 }
             }
             // the cuts inside the item, and so the blocks that share it
-            const int64_t first = ceil_div((s + MIN_UNITS) * blocks, total);
-            const int64_t last = ceil_div((s + n - MIN_UNITS + 1) * blocks, total) - 1;
+            const int first = cuts.from(s + MIN_UNITS);
+            const int last = cuts.from(s + n - MIN_UNITS + 1) - 1;
             __threadfence();
             __syncthreads();
             if (tid == 0) {
@@ -748,10 +816,21 @@ decode_attention_kernel(const Params p) {
             if (whole && have) {
                 __threadfence();
                 j = Joined<FP8>();
-                for (int64_t b = first - 1; b <= last; ++b) {
-                    const Part<D>& q = parts[2 * b + (b == first - 1)];
-                    j.add(__ldcg(&q.m[my_head]), __ldcg(&q.l[my_head]), __ldcg(&q.mv[my_head]),
-                          __ldcg(reinterpret_cast<const float4*>(&q.o[my_head][d4])));
+                constexpr int BATCH = 8;   // parts whose loads are in flight together
+                for (int b = first - 1; b <= last; b += BATCH) {
+                    float m[BATCH], l[BATCH], mv[BATCH];
+                    float4 o[BATCH];
+#pragma unroll
+                    for (int k = 0; k < BATCH; ++k) {
+                        const Part<D>& q = parts[2 * min(b + k, last) + (b + k == first - 1)];
+                        m[k] = __ldcg(&q.m[my_head]);
+                        l[k] = __ldcg(&q.l[my_head]);
+                        mv[k] = FP8 ? __ldcg(&q.mv[my_head]) : 0.0f;
+                        o[k] = __ldcg(reinterpret_cast<const float4*>(&q.o[my_head][d4]));
+                    }
+#pragma unroll
+                    for (int k = 0; k < BATCH; ++k)
+                        if (b + k <= last) j.add(m[k], l[k], mv[k], o[k]);
                 }
             }
         }
@@ -762,10 +841,10 @@ decode_attention_kernel(const Params p) {
 template <int D, bool FP8>
 int launch(const Params& p, int blocks, cudaStream_t stream) {
     static std::atomic<bool> done[MAX_DEVICES];
-    constexpr int bytes = 2 * WARPS * sizeof(Slot<D>);
+    constexpr int bytes = 2 * warps<FP8>() * sizeof(Slot<D>);
     if (!set_smem_once(done, decode_attention_kernel<D, FP8>, bytes))
         return launch_status("qb_decode_attention: shared memory");
-    decode_attention_kernel<D, FP8><<<blocks, WARPS * 32, bytes, stream>>>(p);
+    decode_attention_kernel<D, FP8><<<blocks, warps<FP8>() * 32, bytes, stream>>>(p);
     return launch_status("qb_decode_attention");
 }
 
@@ -776,10 +855,8 @@ int resident_blocks() {
     if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= MAX_DEVICES) return 0;
     int n = cache[dev].load(std::memory_order_acquire);
     if (n == 0) {
-        int sms = 0;
-        if (cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess)
+        if (cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess)
             return 0;
-        n = sms * BLOCKS_PER_SM;
         cache[dev].store(n, std::memory_order_release);
     }
     return n;
@@ -810,8 +887,9 @@ extern "C" int qb_decode_attention(const void* q, int64_t q_ld, int64_t rows, in
     const char* who = "qb_decode_attention";
     if (head_dim != 64 && head_dim != 128)
         return invalid("qb_decode_attention: head_dim must be 64 or 128");
-    if (n_q <= 0 || n_kv <= 0 || n_q % n_kv)
-        return invalid("qb_decode_attention: n_q must be a positive multiple of n_kv");
+    if (n_q <= 0 || n_q > 4096 || n_kv <= 0 || n_q % n_kv)
+        return invalid("qb_decode_attention: n_q must be a positive multiple of n_kv, at most "
+                       "4096");
     if (rows < 0 || rows > 65535) return invalid("qb_decode_attention: 0 to 65,535 rows");
     if (page_tokens < 8 || page_tokens > 1024 || (page_tokens & (page_tokens - 1)))
         return invalid("qb_decode_attention: page_tokens must be a power of two from 8 to 1024");
@@ -834,7 +912,7 @@ extern "C" int qb_decode_attention(const void* q, int64_t q_ld, int64_t rows, in
     if (!aligned(k_pool, 16) || !aligned(v_pool, 16))
         return invalid("qb_decode_attention: the pools must be 16-byte aligned");
     if (n_pages <= 0 || table_width <= 0 || table_ld < table_width ||
-        table_width > 0x7fffffffLL / page_tokens)
+        table_width > (1 << 30) / page_tokens)
         return invalid("qb_decode_attention: bad table width or page count");
     if (!workspace || !aligned(workspace, 16))
         return invalid("qb_decode_attention: the workspace must be 16-byte aligned");
@@ -857,6 +935,10 @@ extern "C" int qb_decode_attention(const void* q, int64_t q_ld, int64_t rows, in
     p.v_scale = v_scale;
     p.n_pages = n_pages;
     p.page_shift = __builtin_ctz((unsigned)page_tokens);
+    // the line of all units, and what is added to a place in it, below 2^31
+    p.unit_shift = UNIT_SHIFT;
+    while (rows * n_kv * p.tiles * ((table_width * page_tokens >> p.unit_shift) + 1) >= 1LL << 30)
+        ++p.unit_shift;
     p.table = table;
     p.table_width = table_width;
     p.table_ld = table_ld;
