@@ -142,6 +142,12 @@ __device__ __forceinline__ uint2 load8(const void* p) {
     return r;
 }
 
+__device__ __forceinline__ float log2_approx(float x) {
+    float r;
+    asm("lg2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
+    return r;
+}
+
 __device__ __forceinline__ float exp2_approx(float x) {
     float r;
     asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
@@ -196,7 +202,8 @@ struct alignas(16) Slot {
     float o[HEADS][D + 4];
     float m[HEADS], l[HEADS], mv[HEADS];
     int start;           // the item's first unit, over all items; -1: no part
-    int n, row, item;    // its units, row and place in the row
+    int n, row;          // its units and row
+    int head0, heads;    // its query heads
     int whole;           // 2: starts the item, 1: ends it
 };
 static_assert(sizeof(Slot<64>) % 16 == 0 && sizeof(Slot<128>) % 16 == 0,
@@ -583,14 +590,14 @@ __device__ __forceinline__ void finish(const Params& p, const Joined<FP8>& j, in
     const float NEG_INF = __uint_as_float(0xFF800000u);
     float r[4] = {0.0f, 0.0f, 0.0f, 0.0f};
     if (j.l != 0.0f) {   // a NaN stays one
-        float f = 1.0f / j.l;
+        float f = __fdividef(1.0f, j.l);
         if (FP8 && j.mv > NEG_INF) f *= exp2f(j.mv - j.m - LIFT);
 #pragma unroll
         for (int i = 0; i < 4; ++i) r[i] = j.acc[i] * f;
     }
     if (live) {
         if (p.lse && d4 == 0)
-            p.lse[row * (int64_t)p.n_q + head] = j.l != 0.0f ? j.m * LN2 + logf(j.l) : NEG_INF;
+            p.lse[row * (int64_t)p.n_q + head] = j.l != 0.0f ? (j.m + log2_approx(j.l)) * LN2 : NEG_INF;
         if (p.out) {
             uint2 b;
             b.x = bf16x2_bits(r[0], r[1]);
@@ -629,43 +636,41 @@ decode_attention_kernel(const Params p) {
     extern __shared__ __align__(16) char smem[];
     Slot<D>* slots = reinterpret_cast<Slot<D>*>(smem);   // [WARPS][2]: begun before, begun here
     __shared__ int s_scan[WARPS], s_full[WARPS];
-    __shared__ Place s_cut[2], s_start[WARPS];
-    __shared__ uint32_t s_last;
+    __shared__ int s_upto[THREADS];   // units of one head through each thread's rows
+    __shared__ uint32_t s_joins[2];
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     const int per_row = p.n_kv * p.tiles;   // items of a row
 
-    // ---- a scan over the rows' units: this thread's rows hold [from, to)
+    // ---- a scan over the rows' units, `chunk` rows a thread
     const int chunk = (p.rows + THREADS - 1) / THREADS;
     const int r0 = min(tid * chunk, p.rows), r1 = min(r0 + chunk, p.rows);
-    int mine = 0, full = 0;
+    int upto = 0, full = 0;
     for (int r = r0; r < r1; ++r) {
         const int n = units_of(p, row_keys(p, r, blockIdx.x == 0));
-        mine += n;
+        upto += n;
         full += n > 0;
     }
-    int upto = mine;
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
         const int u = __shfl_up_sync(0xffffffffu, upto, o);
         if (lane >= o) upto += u;
     }
     full = __reduce_add_sync(0xffffffffu, full);
+    s_upto[tid] = upto;
     if (lane == 31) {
         s_scan[warp] = upto;
         s_full[warp] = full;
     }
     if (lane < 2) slots[2 * warp + lane].start = -1;
     __syncthreads();
-    int units = 0;
+    int units = 0, earlier[WARPS];   // of the warps before each
     full = 0;
 #pragma unroll
     for (int w = 0; w < WARPS; ++w) {
-        if (w < warp) upto += s_scan[w];
+        earlier[w] = units;
         units += s_scan[w];
         full += s_full[w];
     }
-    const int first_unit = upto - mine;   // of one head
-    const int from = first_unit * per_row, to = upto * per_row;
     const int total = units * per_row;
     // rows without keys
     if (full < p.rows)
@@ -680,51 +685,47 @@ decode_attention_kernel(const Params p) {
     const int blocks = min((int)gridDim.x, max(full * per_row, total / MIN_UNITS));
     if ((int)blockIdx.x >= blocks) return;
 
-    // ---- this block's range, and its warps'
-    const Cuts cuts(total, blocks);
-    // the place of unit x, which is one of this thread's; its item's units in n
-    auto place = [&](int x, int& n) {
-        Place at = {x, r0, first_unit};
-        for (; at.row < r1; ++at.row) {
+    // ---- this block's range and this warp's share, each warp for itself
+    // The place of unit x: the threads whose rows end at x or before are
+    // counted, then the next one's rows walked. n: the units of its item.
+    auto locate = [&](int x, int& n) {
+        int ended = 0;
+#pragma unroll
+        for (int w = 0; w < WARPS; ++w)
+            ended += (earlier[w] + s_upto[32 * w + lane]) * per_row <= x;
+        ended = __reduce_add_sync(0xffffffffu, ended);
+        Place at = {x, ended * chunk, 0};
+        if (ended) {
+            at.before = s_upto[ended - 1];
+#pragma unroll
+            for (int w = 0; w < WARPS; ++w)
+                if ((ended - 1) >> 5 == w) at.before += earlier[w];
+        }
+        for (;; ++at.row) {
             n = units_of(p, row_keys(p, at.row, false));
-            if (x < (at.before + n) * per_row) break;
+            if (x < (at.before + n) * per_row) return at;
             at.before += n;
         }
-        return at;
     };
-#pragma unroll
-    for (int c = 0; c < 2; ++c) {
-        const int i = blockIdx.x + c;
+    const Cuts cuts(total, blocks);
+    auto cut = [&](int i) {
+        if (i == blocks) return total;
         const int x = cuts.at(i);
-        if (x >= from && x < to) {
-            int n;
-            Place at = place(x, n);
-            const int s = at.before * per_row;
-            at.at = settle(x, s + (x - s) / n * n, n);
-            s_cut[c] = at;
-        }
-        if (i == blocks && tid == 0) s_cut[c].at = total;
-    }
-    __syncthreads();
-    const int lo = s_cut[0].at, hi = s_cut[1].at;
-    if (lo == hi) return;   // an item that a neighbour has whole
+        int n;
+        const Place at = locate(x, n);
+        const int s = at.before * per_row;
+        return settle(x, s + (x - s) / n * n, n);
+    };
+    const int lo = cut(blockIdx.x), hi = cut(blockIdx.x + 1);
     const Cuts shares(hi - lo, WARPS);
-    if (from < hi && to > lo) {
-#pragma unroll
-        for (int w = 0; w < WARPS; ++w) {
-            const int x = lo + shares.at(w);
-            int n;
-            if (x >= from && x < to) s_start[w] = place(x, n);
-        }
-    }
-    __syncthreads();
 
     // ---- this warp's range, an item after another
     int at = lo + shares.at(warp);
     const int end = lo + shares.at(warp + 1);
     if (at < end) {
-        int row = s_start[warp].row, before = s_start[warp].before;
-        int keys = row_keys(p, row, false), n = units_of(p, keys);
+        int n;
+        const Place begin = locate(at, n);
+        int row = begin.row, before = begin.before, keys = row_keys(p, row, false);
         for (;;) {
             const int item = (at - before * per_row) / n;
             const int s = before * per_row + item * n;
@@ -750,7 +751,8 @@ decode_attention_kernel(const Params p) {
                 slot.start = s;
                 slot.n = n;
                 slot.row = row;
-                slot.item = item;
+                slot.head0 = head0;
+                slot.heads = heads;
                 slot.whole = whole;
             }
             __syncwarp();
@@ -766,75 +768,91 @@ decode_attention_kernel(const Params p) {
     }
     __syncthreads();
 
-    // ---- the parts that warps share, in order
-    const int my_head = tid / QUADS, d4 = tid % QUADS * 4;
-    const bool have = my_head < HEADS;   // the threads past the heads' columns help nothing
+    // ---- the parts that warps share, in order: a chain of parts an item, a
+    // warp for each chain and head (two heads, D = 64)
+    constexpr int PASSES = HEADS * QUADS / 32;
+    const int d4 = lane % QUADS * 4;
     const int start = lane < 2 * WARPS ? slots[lane].start : -1;
-    uint32_t left = __ballot_sync(0xffffffffu, start >= 0);
-    while (left) {
-        const int i = __ffs(left) - 1;
-        const int s = __shfl_sync(0xffffffffu, start, i);
-        uint32_t chain = __ballot_sync(0xffffffffu, start == s);
-        left &= ~chain;
-        const int row = slots[i].row, item = slots[i].item, n = slots[i].n;
-        const int kvh = item / p.tiles, tile = item % p.tiles;
-        const int head0 = kvh * p.group + tile * HEADS;
-        const int heads = min(HEADS, p.group - tile * HEADS);
-        const bool begins = slots[i].whole & 2;
-        bool whole = begins && (slots[31 - __clz(chain)].whole & 1);
-        Joined<FP8> j;
-        if (have)
-            for (; chain; chain &= chain - 1) {
-                const Slot<D>& slot = slots[__ffs(chain) - 1];
-                j.add(slot.m[my_head], slot.l[my_head], slot.mv[my_head],
-                      *reinterpret_cast<const float4*>(&slot.o[my_head][d4]));
+    const uint32_t same = __match_any_sync(0xffffffffu, start);
+    const bool leads = start >= 0 && (same & ((1u << lane) - 1u)) == 0;
+    bool parted = false;   // the chain is not its whole item
+    if (leads) parted = !(slots[lane].whole & 2) || !(slots[31 - __clz(same)].whole & 1);
+    uint32_t chains = __ballot_sync(0xffffffffu, leads);
+    const uint32_t open = __ballot_sync(0xffffffffu, parted);   // two at most
+    Part<D>* parts = (Part<D>*)p.parts;
+    for (int i = warp; chains; i -= PASSES, chains &= chains - 1) {
+        const int lead = __ffs(chains) - 1;
+        const uint32_t chain = __shfl_sync(0xffffffffu, same, lead);
+        for (; i < PASSES; i += WARPS) {
+            const int head = i * (32 / QUADS) + lane / QUADS;
+            Joined<FP8> j;
+            for (uint32_t c = chain; c; c &= c - 1) {
+                const Slot<D>& slot = slots[__ffs(c) - 1];
+                j.add(slot.m[head], slot.l[head], slot.mv[head],
+                      *reinterpret_cast<const float4*>(&slot.o[head][d4]));
             }
-        if (!whole) {
-            Part<D>* parts = (Part<D>*)p.parts;
-            Part<D>& part = parts[2 * blockIdx.x + begins];
-            if (have) {
-                __stcg(reinterpret_cast<float4*>(&part.o[my_head][d4]),
+            const Slot<D>& slot = slots[lead];
+            if (open >> lead & 1) {
+                Part<D>& part = parts[2 * blockIdx.x + (slot.whole >> 1)];
+                __stcg(reinterpret_cast<float4*>(&part.o[head][d4]),
                        make_float4(j.acc[0], j.acc[1], j.acc[2], j.acc[3]));
                 if (d4 == 0) {
-                    __stcg(&part.m[my_head], j.m);
-                    __stcg(&part.l[my_head], j.l);
-                    __stcg(&part.mv[my_head], j.mv);
+                    __stcg(&part.m[head], j.m);
+                    __stcg(&part.l[head], j.l);
+                    __stcg(&part.mv[head], j.mv);
                 }
-            }
-            // the cuts inside the item, and so the blocks that share it
-            const int first = cuts.from(s + MIN_UNITS);
-            const int last = cuts.from(s + n - MIN_UNITS + 1) - 1;
-            __threadfence();
-            __syncthreads();
-            if (tid == 0) {
-                const uint32_t others = atomicAdd(p.arrived + first, 1u);
-                s_last = others == (uint32_t)(last - first + 1);
-                if (s_last) p.arrived[first] = 0;   // for the next launch
-            }
-            __syncthreads();
-            whole = s_last;
-            if (whole && have) {
-                __threadfence();
-                j = Joined<FP8>();
-                constexpr int BATCH = 8;   // parts whose loads are in flight together
-                for (int b = first - 1; b <= last; b += BATCH) {
-                    float m[BATCH], l[BATCH], mv[BATCH];
-                    float4 o[BATCH];
-#pragma unroll
-                    for (int k = 0; k < BATCH; ++k) {
-                        const Part<D>& q = parts[2 * min(b + k, last) + (b + k == first - 1)];
-                        m[k] = __ldcg(&q.m[my_head]);
-                        l[k] = __ldcg(&q.l[my_head]);
-                        mv[k] = FP8 ? __ldcg(&q.mv[my_head]) : 0.0f;
-                        o[k] = __ldcg(reinterpret_cast<const float4*>(&q.o[my_head][d4]));
-                    }
-#pragma unroll
-                    for (int k = 0; k < BATCH; ++k)
-                        if (b + k <= last) j.add(m[k], l[k], mv[k], o[k]);
-                }
+            } else {
+                finish<D, FP8>(p, j, slot.row, slot.head0 + head, head < slot.heads, d4);
             }
         }
-        if (whole && have) finish<D, FP8>(p, j, row, head0 + my_head, my_head < heads, d4);
+    }
+    if (!open) return;
+
+    // ---- the parts that blocks share: the last to arrive joins them
+    __threadfence();
+    __syncthreads();
+    auto sharers = [&](const Slot<D>& slot, int& first, int& last) {   // the cuts inside the item
+        first = cuts.from(slot.start + MIN_UNITS);
+        last = cuts.from(slot.start + slot.n - MIN_UNITS + 1) - 1;
+    };
+    if (tid < __popc(open)) {
+        const uint32_t which = tid == 0 ? open : open & (open - 1);
+        int first, last;
+        sharers(slots[__ffs(which) - 1], first, last);
+        const uint32_t others = atomicAdd(p.arrived + first, 1u);
+        const bool all = others == (uint32_t)(last - first + 1);
+        if (all) p.arrived[first] = 0;   // for the next launch
+        __threadfence();
+        s_joins[tid] = all;
+    }
+    __syncthreads();
+    uint32_t which = open;
+    for (int k = 0; which; ++k, which &= which - 1) {
+        if (!s_joins[k]) continue;
+        const Slot<D>& slot = slots[__ffs(which) - 1];
+        int first, last;
+        sharers(slot, first, last);
+        for (int i = warp; i < PASSES; i += WARPS) {
+            const int head = i * (32 / QUADS) + lane / QUADS;
+            Joined<FP8> j;
+            constexpr int BATCH = 8;   // parts whose loads are in flight together
+            for (int b = first - 1; b <= last; b += BATCH) {
+                float m[BATCH], l[BATCH], mv[BATCH];
+                float4 o[BATCH];
+#pragma unroll
+                for (int u = 0; u < BATCH; ++u) {
+                    const Part<D>& part = parts[2 * min(b + u, last) + (b + u == first - 1)];
+                    m[u] = __ldcg(&part.m[head]);
+                    l[u] = __ldcg(&part.l[head]);
+                    mv[u] = FP8 ? __ldcg(&part.mv[head]) : 0.0f;
+                    o[u] = __ldcg(reinterpret_cast<const float4*>(&part.o[head][d4]));
+                }
+#pragma unroll
+                for (int u = 0; u < BATCH; ++u)
+                    if (b + u <= last) j.add(m[u], l[u], mv[u], o[u]);
+            }
+            finish<D, FP8>(p, j, slot.row, slot.head0 + head, head < slot.heads, d4);
+        }
     }
 }
 
