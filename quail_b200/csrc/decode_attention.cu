@@ -46,7 +46,7 @@ constexpr int WHOLE_UNITS = 16;       // items up to this long are not cut
 // Warps of a block, one block an SM.
 template <bool FP8>
 constexpr int warps() {
-    return FP8 ? 8 : 12;
+    return FP8 ? 8 : 10;
 }
 constexpr float LN2 = 0.693147180559945309f;
 constexpr float LOG2E = 1.44269504088896341f;
@@ -154,11 +154,11 @@ __device__ __forceinline__ float exp2_approx(float x) {
     return r;
 }
 
-// e4m3 pair (low half of c) -> f16 pair, exactly
-__device__ __forceinline__ uint32_t e4m3x2_f16x2(uint32_t c) {
-    uint32_t r;
-    asm("cvt.rn.f16x2.e4m3x2 %0, %1;" : "=r"(r) : "h"((uint16_t)c));
-    return r;
+// four e4m3 codes -> two f16 pairs (codes 0, 1 and 2, 3), exactly
+__device__ __forceinline__ void e4m3x4_f16(uint32_t c, uint32_t& a, uint32_t& b) {
+    asm("{.reg .b16 l, h; mov.b32 {l, h}, %2;\n\t"
+        "cvt.rn.f16x2.e4m3x2 %0, l;\n\tcvt.rn.f16x2.e4m3x2 %1, h;}"
+        : "=r"(a), "=r"(b) : "r"(c));
 }
 
 template <bool F16>
@@ -294,96 +294,103 @@ __device__ __forceinline__ void attend(const Params& p, Slot<D>& slot, int row, 
     // A step: 16 keys of 128 bf16, else 32. The pipeline: while a step is
     // computed, the next one's K (as soon as S has consumed the registers), V
     // (after the second product) and, one further, the page ids are on their
-    // way.
+    // way. Keys past the end are taken as the last one, with a weight of zero.
     constexpr int UNITS = FP8 || D == 64 ? 2 : 1;
-    const int64_t row_bytes = (int64_t)p.n_kv * D * ELEM;
-    const int64_t page_bytes = row_bytes << p.page_shift;
-    const char* k_lane = (const char*)p.k + (int64_t)kvh * D * ELEM + g * row_bytes + t * 16;
-    const char* v_lane = (const char*)p.v + (int64_t)kvh * D * ELEM + 2 * t * row_bytes +
-                         g * (FP8 && D == 64 ? 8 : 16);
-    const int n_pages = (int)min(p.n_pages, (int64_t)0x7fffffff);
-    const int mask = (1 << p.page_shift) - 1;
+    constexpr int STEP = 16 * UNITS;
+    const uint32_t row_bytes = (uint32_t)p.n_kv * (D * ELEM);
+    const char* k_lane = (const char*)p.k + kvh * D * ELEM + t * 16;
+    const char* v_lane = (const char*)p.v + kvh * D * ELEM + g * (FP8 && D == 64 ? 8 : 16);
+    const uint32_t mask = (1u << p.page_shift) - 1u, n_pages = (uint32_t)p.n_pages;
 
     uint4 kr[UNITS][2][KC], vr[UNITS][4][VC];
     uint32_t kb[UNITS][2], vb[UNITS][2];   // 8 bit: exponent bytes of keys g and g + 8
-    int ids[UNITS][2];                     // pages of the half steps, -1: none
-    // a page holds a multiple of 8 tokens, so each half step is in one page
-    auto find = [&](int key0) {
+    // the next step's keys g and g + 8 of each unit: page ids, then pool rows
+    uint32_t rows[UNITS][2];
+    uint32_t lost = 0, next_lost = 0;      // bit 2u + h: the key's page is out of range
+    auto find = [&](int from) {
 #pragma unroll
         for (int u = 0; u < UNITS; ++u)
 #pragma unroll
             for (int h = 0; h < 2; ++h) {
-                const int key = key0 + 16 * u + 8 * h;
-                ids[u][h] = key < end ? __ldg(table + (key >> p.page_shift)) : -1;
+                const int key = min(from + 16 * u + 8 * h + g, end - 1);
+                rows[u][h] = (uint32_t)__ldg(table + (key >> p.page_shift));
             }
     };
-    auto check = [&](int key0) {
-#pragma unroll
-        for (int u = 0; u < UNITS; ++u)
-#pragma unroll
-            for (int h = 0; h < 2; ++h)
-                if ((uint32_t)ids[u][h] >= (uint32_t)n_pages) {
-                    if (key0 + 16 * u + 8 * h < end && lane == 0)
-                        atomicOr(p.status, STATUS_BAD_INDEX);
-                    ids[u][h] = -1;
-                }
-    };
-    // bit 2u + h: key g of that half step is one
-    auto load_k = [&](int key0) {
-        uint32_t ok = 0;
+    auto load_k = [&](int from) {
+        next_lost = 0;
 #pragma unroll
         for (int u = 0; u < UNITS; ++u)
 #pragma unroll
             for (int h = 0; h < 2; ++h) {
-                const int key = key0 + 16 * u + 8 * h;
-                const bool in = ids[u][h] >= 0 && key + g < end;
-                const char* at = k_lane + ids[u][h] * page_bytes + (key & mask) * row_bytes;
-                ok |= in ? 1u << (2 * u + h) : 0u;
+                const uint32_t key = (uint32_t)min(from + 16 * u + 8 * h + g, end - 1);
+                const uint32_t id = rows[u][h];
+                rows[u][h] = (id << p.page_shift) + (key & mask);
+                if (id >= n_pages) {
+                    rows[u][h] = 0;
+                    next_lost |= 1u << (2 * u + h);
+                }
+                const char* at = k_lane + (uint64_t)rows[u][h] * row_bytes;
 #pragma unroll
-                for (int c = 0; c < KC; ++c)
-                    kr[u][h][c] = in ? load16(at + 64 * c) : make_uint4(0, 0, 0, 0);
+                for (int c = 0; c < KC; ++c) kr[u][h][c] = load16(at + 64 * c);
                 if (FP8) {
-                    const int64_t row =
-                        ((int64_t)ids[u][h] << p.page_shift) + (key & mask) + g;
-                    kb[u][h] = in ? p.k_scale[row * p.n_kv + kvh] : 127u;
-                    vb[u][h] = in ? p.v_scale[row * p.n_kv + kvh] : 127u;
+                    const uint64_t head = (uint64_t)rows[u][h] * (uint32_t)p.n_kv + kvh;
+                    kb[u][h] = __ldg(p.k_scale + head);
+                    vb[u][h] = __ldg(p.v_scale + head);
                 }
             }
-        return ok;
     };
-    // V: rows 2t, 2t + 1 of each half; keys past the end are zeros, for
-    // 0 * NaN is NaN
-    auto load_v = [&](int key0) {
+    // V: keys 2t, 2t + 1 of each half
+    auto load_v = [&]() {
 #pragma unroll
         for (int u = 0; u < UNITS; ++u)
 #pragma unroll
             for (int r = 0; r < 4; ++r) {
-                const int h = r >> 1, key = key0 + 16 * u + 8 * h;
-                const bool in = ids[u][h] >= 0 && key + 2 * t + (r & 1) < end;
-                const char* at = v_lane + ids[u][h] * page_bytes +
-                                 ((key & mask) + (r & 1)) * row_bytes;
+                const uint32_t row =
+                    __shfl_sync(0xffffffffu, rows[u][r >> 1], 8 * t + 4 * (r & 1));
+                const char* at = v_lane + (uint64_t)row * row_bytes;
 #pragma unroll
                 for (int c = 0; c < VC; ++c) {
-                    vr[u][r][c] = make_uint4(0, 0, 0, 0);
                     if (FP8 && D == 64) {
-                        if (in) {
-                            const uint2 w = load8(at);
-                            vr[u][r][c].x = w.x;
-                            vr[u][r][c].y = w.y;
-                        }
-                    } else if (in) {
+                        const uint2 w = load8(at);
+                        vr[u][r][c] = make_uint4(w.x, w.y, 0, 0);
+                    } else {
                         vr[u][r][c] = load16(at + 128 * c);
                     }
                 }
             }
+        if (__any_sync(0xffffffffu, next_lost)) {   // 0 * NaN is NaN
+            if (lane == 0) atomicOr(p.status, STATUS_BAD_INDEX);
+#pragma unroll
+            for (int u = 0; u < UNITS; ++u)
+#pragma unroll
+                for (int r = 0; r < 4; ++r) {
+                    const uint32_t l =
+                        __shfl_sync(0xffffffffu, next_lost, 8 * t + 4 * (r & 1));
+                    if (l >> (2 * u + (r >> 1)) & 1)
+#pragma unroll
+                        for (int c = 0; c < VC; ++c) vr[u][r][c] = make_uint4(0, 0, 0, 0);
+                }
+        }
     };
 
     find(key0);
-    check(key0);
-    uint32_t k_ok = load_k(key0);
-    load_v(key0);
-    find(key0 + 16 * UNITS);
-    for (; key0 < end; key0 += 16 * UNITS) {
+    load_k(key0);
+    load_v();
+    lost = next_lost;
+    find(key0 + STEP);
+    for (; key0 < end; key0 += STEP) {
+        // the scales of keys g and g + 8: a factor, and (values) an exponent,
+        // the byte as a float by way of a mantissa
+        float by[UNITS][2], more[UNITS][2];
+        if (FP8)
+#pragma unroll
+            for (int u = 0; u < UNITS; ++u)
+#pragma unroll
+                for (int h = 0; h < 2; ++h) {
+                    by[u][h] = e8m0_float(kb[u][h]);
+                    more[u][h] = __uint_as_float(0x4B000000u | vb[u][h]) - 8388735.0f;
+                    if (vb[u][h] == 255u) more[u][h] = __uint_as_float(0x7FFFFFFFu);
+                }
         // ---- S^T: keys g and g + 8, heads 2t and 2t + 1
         float s[UNITS][4];
 #pragma unroll
@@ -398,10 +405,13 @@ __device__ __forceinline__ void attend(const Params& p, Slot<D>& slot, int row, 
                                         kr[u][1][c].w};
                 if (FP8) {
 #pragma unroll
-                    for (int w = 0; w < 4; ++w)
-                        mma16816<true>(s[u], e4m3x2_f16x2(w0[w]), e4m3x2_f16x2(w1[w]),
-                                       e4m3x2_f16x2(w0[w] >> 16), e4m3x2_f16x2(w1[w] >> 16),
-                                       qf[8 * c + 2 * w], qf[8 * c + 2 * w + 1]);
+                    for (int w = 0; w < 4; ++w) {
+                        uint32_t a0, a1, a2, a3;
+                        e4m3x4_f16(w0[w], a0, a2);
+                        e4m3x4_f16(w1[w], a1, a3);
+                        mma16816<true>(s[u], a0, a1, a2, a3, qf[8 * c + 2 * w],
+                                       qf[8 * c + 2 * w + 1]);
+                    }
                 } else {
 #pragma unroll
                     for (int w = 0; w < 2; ++w)
@@ -410,34 +420,41 @@ __device__ __forceinline__ void attend(const Params& p, Slot<D>& slot, int row, 
                 }
             }
         }
-        float x[UNITS][4], y[UNITS][4];   // [2 * half + head]; y: x and the value's exponent
-        bool raise = false;
+        const uint32_t now_lost = lost;
+        load_k(key0 + STEP);   // (past the end: the last key again)
+        // x, and y = x and the value's exponent: [2 * half + head]
+        float x[UNITS][4], y[UNITS][4];
 #pragma unroll
         for (int u = 0; u < UNITS; ++u)
 #pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                float v = s[u][i] * x_scale[i & 1];
-                if (FP8) v *= e8m0_float(kb[u][i >> 1]);
-                if (!(k_ok >> (2 * u + (i >> 1)) & 1)) v = NEG_INF;
-                x[u][i] = y[u][i] = v;
-                raise |= v > top[i & 1] + SLACK;
-                if (FP8) {
-                    const uint32_t b = vb[u][i >> 1];
-                    y[u][i] += b == 255u ? __uint_as_float(0x7FFFFFFFu) : (float)((int)b - 127);
-                    raise |= y[u][i] > top_v[i & 1] + SLACK;
+            for (int h = 0; h < 2; ++h) {
+                const bool in =
+                    key0 + 16 * u + 8 * h + g < end && !(now_lost >> (2 * u + h) & 1);
+#pragma unroll
+                for (int n = 0; n < 2; ++n) {
+                    const float z =
+                        s[u][2 * h + n] * (FP8 ? by[u][h] * x_scale[n] : x_scale[n]);
+                    x[u][2 * h + n] = in ? z : NEG_INF;
+                    y[u][2 * h + n] = FP8 ? x[u][2 * h + n] + more[u][h] : 0.0f;
                 }
             }
-        check(key0 + 16 * UNITS);
-        k_ok = load_k(key0 + 16 * UNITS);
+        float most[2], most_v[2];
+#pragma unroll
+        for (int n = 0; n < 2; ++n) {
+            most[n] = fmaxf(x[0][n], x[0][2 + n]);
+            most_v[n] = fmaxf(y[0][n], y[0][2 + n]);
+#pragma unroll
+            for (int u = 1; u < UNITS; ++u) {
+                most[n] = fmax3(most[n], x[u][n], x[u][2 + n]);
+                most_v[n] = fmax3(most_v[n], y[u][n], y[u][2 + n]);
+            }
+        }
+        bool raise = most[0] > top[0] + SLACK || most[1] > top[1] + SLACK;
+        if (FP8) raise |= most_v[0] > top_v[0] + SLACK || most_v[1] > top_v[1] + SLACK;
         if (__any_sync(0xffffffffu, raise)) {
 #pragma unroll
             for (int n = 0; n < 2; ++n) {
-                float a = top[n], b = top_v[n];
-#pragma unroll
-                for (int u = 0; u < UNITS; ++u) {
-                    a = fmax3(a, x[u][n], x[u][2 + n]);
-                    b = fmax3(b, y[u][n], y[u][2 + n]);
-                }
+                float a = fmaxf(top[n], most[n]), b = fmaxf(top_v[n], most_v[n]);
 #pragma unroll
                 for (int off = 4; off < 32; off <<= 1) {
                     a = fmaxf(a, __shfl_xor_sync(0xffffffffu, a, off));
@@ -507,10 +524,13 @@ __device__ __forceinline__ void attend(const Params& p, Slot<D>& slot, int row, 
                         const uint32_t a23 = __byte_perm(v[0][i], v[1][i], 0x7362);
                         const uint32_t b01 = __byte_perm(v[2][i], v[3][i], 0x5140);
                         const uint32_t b23 = __byte_perm(v[2][i], v[3][i], 0x7362);
-                        mma16816<true>(o[2 * i], e4m3x2_f16x2(a01), e4m3x2_f16x2(a01 >> 16),
-                                       e4m3x2_f16x2(b01), e4m3x2_f16x2(b01 >> 16), hi[0], hi[1]);
-                        mma16816<true>(o[2 * i + 1], e4m3x2_f16x2(a23), e4m3x2_f16x2(a23 >> 16),
-                                       e4m3x2_f16x2(b23), e4m3x2_f16x2(b23 >> 16), hi[0], hi[1]);
+                        uint32_t f[8];
+                        e4m3x4_f16(a01, f[0], f[1]);
+                        e4m3x4_f16(b01, f[2], f[3]);
+                        e4m3x4_f16(a23, f[4], f[5]);
+                        e4m3x4_f16(b23, f[6], f[7]);
+                        mma16816<true>(o[2 * i], f[0], f[1], f[2], f[3], hi[0], hi[1]);
+                        mma16816<true>(o[2 * i + 1], f[4], f[5], f[6], f[7], hi[0], hi[1]);
                     } else {
                         const uint32_t a0 = __byte_perm(v[0][i], v[1][i], 0x5410);
                         const uint32_t a1 = __byte_perm(v[0][i], v[1][i], 0x7632);
@@ -522,8 +542,9 @@ __device__ __forceinline__ void attend(const Params& p, Slot<D>& slot, int row, 
                 }
             }
         }
-        load_v(key0 + 16 * UNITS);
-        find(key0 + 32 * UNITS);
+        lost = next_lost;
+        load_v();
+        find(key0 + 2 * STEP);
     }
 
     // ---- the warp's sums, and its state to shared memory
@@ -549,8 +570,8 @@ __device__ __forceinline__ void attend(const Params& p, Slot<D>& slot, int row, 
     }
 }
 
-// Four columns of one head, as the join accumulates them: parts with their
-// own exponents, brought to the largest.
+// Four columns of one head, joined from parts with their own exponents, which
+// are brought to the largest.
 template <bool FP8>
 struct Joined {
     float m, mv, l, acc[4];
@@ -558,26 +579,35 @@ struct Joined {
         m = mv = __uint_as_float(0xFF800000u);
         l = acc[0] = acc[1] = acc[2] = acc[3] = 0.0f;
     }
-    // x against the exponent `from`, brought to `to`; nothing has `from` -inf
+    // 2^(from - to); nothing has `from` -inf
     static __device__ __forceinline__ float factor(float from, float to) {
         return from > __uint_as_float(0xFF800000u) ? exp2_approx(from - to) : 0.0f;
     }
-    __device__ __forceinline__ void add(float mi, float li, float mvi, const float4& part) {
-        const float top = fmaxf(m, mi);
+    // Up to 32 more parts of the head: lane i holds part i's exponents and sum
+    // (-inf and 0: no part); then add() takes their columns.
+    float f;   // the factor of the lane's part
+    __device__ __forceinline__ void begin(float mi, float li, float mvi) {
+        const float top = fmaxf(m, warp_max(mi));
         const float a = factor(m, top), b = factor(mi, top);
-        l = l * a + li * b;
+        l = l * a + warp_sum(li * b);
         m = top;
-        float fa = a, fb = b;
+        float before = a;
+        f = b;
         if (FP8) {
-            const float top_v = fmaxf(mv, mvi);
-            fa = factor(mv, top_v);
-            fb = factor(mvi, top_v);
+            const float top_v = fmaxf(mv, warp_max(mvi));
+            before = factor(mv, top_v);
+            f = factor(mvi, top_v);
             mv = top_v;
         }
-        acc[0] = acc[0] * fa + part.x * fb;
-        acc[1] = acc[1] * fa + part.y * fb;
-        acc[2] = acc[2] * fa + part.z * fb;
-        acc[3] = acc[3] * fa + part.w * fb;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) acc[i] *= before;
+    }
+    __device__ __forceinline__ void add(int lane, const float4& part) {
+        const float by = __shfl_sync(0xffffffffu, f, lane);
+        acc[0] += part.x * by;
+        acc[1] += part.y * by;
+        acc[2] += part.z * by;
+        acc[3] += part.w * by;
     }
 };
 
@@ -743,8 +773,11 @@ decode_attention_kernel(const Params p) {
                     const int head = i / QUADS, d4 = i % QUADS * 4;
                     if (D == 128 && head >= heads) break;   // D = 64: two heads at a time
                     Joined<FP8> j;
-                    j.add(slot.m[head], slot.l[head], slot.mv[head],
-                          *reinterpret_cast<const float4*>(&slot.o[head][d4]));
+                    j.m = slot.m[head];
+                    j.l = slot.l[head];
+                    j.mv = slot.mv[head];
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) j.acc[e] = slot.o[head][d4 + e];
                     finish<D, FP8>(p, j, row, head0 + head, head < heads, d4);
                 }
             } else if (lane == 0) {
@@ -769,9 +802,11 @@ decode_attention_kernel(const Params p) {
     __syncthreads();
 
     // ---- the parts that warps share, in order: a chain of parts an item, a
-    // warp for each chain and head (two heads, D = 64)
-    constexpr int PASSES = HEADS * QUADS / 32;
+    // warp for each chain and head
+    const float NEG_INF = __uint_as_float(0xFF800000u);
+    const float4 zeros = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
     const int d4 = lane % QUADS * 4;
+    const bool have = lane < QUADS;   // D = 64: half of the lanes have columns
     const int start = lane < 2 * WARPS ? slots[lane].start : -1;
     const uint32_t same = __match_any_sync(0xffffffffu, start);
     const bool leads = start >= 0 && (same & ((1u << lane) - 1u)) == 0;
@@ -780,28 +815,30 @@ decode_attention_kernel(const Params p) {
     uint32_t chains = __ballot_sync(0xffffffffu, leads);
     const uint32_t open = __ballot_sync(0xffffffffu, parted);   // two at most
     Part<D>* parts = (Part<D>*)p.parts;
-    for (int i = warp; chains; i -= PASSES, chains &= chains - 1) {
+    for (int head = warp; chains; head -= HEADS, chains &= chains - 1) {
         const int lead = __ffs(chains) - 1;
         const uint32_t chain = __shfl_sync(0xffffffffu, same, lead);
-        for (; i < PASSES; i += WARPS) {
-            const int head = i * (32 / QUADS) + lane / QUADS;
+        for (; head < HEADS; head += WARPS) {
             Joined<FP8> j;
+            const bool mine = chain >> lane & 1;
+            j.begin(mine ? slots[lane].m[head] : NEG_INF, mine ? slots[lane].l[head] : 0.0f,
+                    mine ? slots[lane].mv[head] : NEG_INF);
             for (uint32_t c = chain; c; c &= c - 1) {
-                const Slot<D>& slot = slots[__ffs(c) - 1];
-                j.add(slot.m[head], slot.l[head], slot.mv[head],
-                      *reinterpret_cast<const float4*>(&slot.o[head][d4]));
+                const int i = __ffs(c) - 1;
+                j.add(i, *reinterpret_cast<const float4*>(&slots[i].o[head][d4]));
             }
             const Slot<D>& slot = slots[lead];
             if (open >> lead & 1) {
                 Part<D>& part = parts[2 * blockIdx.x + (slot.whole >> 1)];
-                __stcg(reinterpret_cast<float4*>(&part.o[head][d4]),
-                       make_float4(j.acc[0], j.acc[1], j.acc[2], j.acc[3]));
-                if (d4 == 0) {
+                if (have)
+                    __stcg(reinterpret_cast<float4*>(&part.o[head][d4]),
+                           make_float4(j.acc[0], j.acc[1], j.acc[2], j.acc[3]));
+                if (lane == 0) {
                     __stcg(&part.m[head], j.m);
                     __stcg(&part.l[head], j.l);
                     __stcg(&part.mv[head], j.mv);
                 }
-            } else {
+            } else if (have) {
                 finish<D, FP8>(p, j, slot.row, slot.head0 + head, head < slot.heads, d4);
             }
         }
@@ -809,7 +846,6 @@ decode_attention_kernel(const Params p) {
     if (!open) return;
 
     // ---- the parts that blocks share: the last to arrive joins them
-    __threadfence();
     __syncthreads();
     auto sharers = [&](const Slot<D>& slot, int& first, int& last) {   // the cuts inside the item
         first = cuts.from(slot.start + MIN_UNITS);
@@ -819,10 +855,11 @@ decode_attention_kernel(const Params p) {
         const uint32_t which = tid == 0 ? open : open & (open - 1);
         int first, last;
         sharers(slots[__ffs(which) - 1], first, last);
+        __threadfence();   // the block's parts, before the count
         const uint32_t others = atomicAdd(p.arrived + first, 1u);
         const bool all = others == (uint32_t)(last - first + 1);
         if (all) p.arrived[first] = 0;   // for the next launch
-        __threadfence();
+        __threadfence();   // the count, before the others' parts
         s_joins[tid] = all;
     }
     __syncthreads();
@@ -832,26 +869,36 @@ decode_attention_kernel(const Params p) {
         const Slot<D>& slot = slots[__ffs(which) - 1];
         int first, last;
         sharers(slot, first, last);
-        for (int i = warp; i < PASSES; i += WARPS) {
-            const int head = i * (32 / QUADS) + lane / QUADS;
+        for (int head = warp; head < HEADS; head += WARPS) {
             Joined<FP8> j;
-            constexpr int BATCH = 8;   // parts whose loads are in flight together
-            for (int b = first - 1; b <= last; b += BATCH) {
-                float m[BATCH], l[BATCH], mv[BATCH];
+            for (int b = first - 1; b <= last; b += 32) {   // a part a lane
+                const int mine = b + lane;
+                const bool in = mine <= last;
+                const Part<D>& part = parts[2 * min(mine, last) + (mine == first - 1)];
+                const float m = in ? __ldcg(&part.m[head]) : NEG_INF;
+                const float l = in ? __ldcg(&part.l[head]) : 0.0f;
+                const float mv = in ? __ldcg(&part.mv[head]) : NEG_INF;
+                constexpr int BATCH = 8;   // parts whose columns are in flight together
                 float4 o[BATCH];
+                auto fetch = [&](int i) {
 #pragma unroll
-                for (int u = 0; u < BATCH; ++u) {
-                    const Part<D>& part = parts[2 * min(b + u, last) + (b + u == first - 1)];
-                    m[u] = __ldcg(&part.m[head]);
-                    l[u] = __ldcg(&part.l[head]);
-                    mv[u] = FP8 ? __ldcg(&part.mv[head]) : 0.0f;
-                    o[u] = __ldcg(reinterpret_cast<const float4*>(&part.o[head][d4]));
+                    for (int u = 0; u < BATCH; ++u) {
+                        const int at = b + i + u;
+                        o[u] = at <= last ? __ldcg(reinterpret_cast<const float4*>(
+                                                &parts[2 * at + (at == first - 1)].o[head][d4]))
+                                          : zeros;
+                    }
+                };
+                fetch(0);
+                j.begin(m, l, mv);
+                for (int i = 0; i < 32 && b + i <= last; i += BATCH) {
+                    if (i) fetch(i);
+#pragma unroll
+                    for (int u = 0; u < BATCH; ++u) j.add(i + u, o[u]);
                 }
-#pragma unroll
-                for (int u = 0; u < BATCH; ++u)
-                    if (b + u <= last) j.add(m[u], l[u], mv[u], o[u]);
             }
-            finish<D, FP8>(p, j, slot.row, slot.head0 + head, head < slot.heads, d4);
+            if (have)
+                finish<D, FP8>(p, j, slot.row, slot.head0 + head, head < slot.heads, d4);
         }
     }
 }
@@ -932,6 +979,8 @@ extern "C" int qb_decode_attention(const void* q, int64_t q_ld, int64_t rows, in
     if (n_pages <= 0 || table_width <= 0 || table_ld < table_width ||
         table_width > (1 << 30) / page_tokens)
         return invalid("qb_decode_attention: bad table width or page count");
+    if (n_pages >= (1LL << 31) || n_pages * page_tokens >= (1LL << 32))
+        return invalid("qb_decode_attention: the pools have 2^32 rows or more");
     if (!workspace || !aligned(workspace, 16))
         return invalid("qb_decode_attention: the workspace must be 16-byte aligned");
     const int blocks = resident_blocks();
