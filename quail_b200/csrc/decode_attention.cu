@@ -148,6 +148,13 @@ __device__ __forceinline__ float log2_approx(float x) {
     return r;
 }
 
+// the largest of a warp's values (NaN passed over)
+__device__ __forceinline__ float redux_max(float x) {
+    float r;
+    asm("redux.sync.max.f32 %0, %1, 0xffffffff;" : "=f"(r) : "f"(x));
+    return r;
+}
+
 __device__ __forceinline__ float exp2_approx(float x) {
     float r;
     asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
@@ -587,14 +594,14 @@ struct Joined {
     // (-inf and 0: no part); then add() takes their columns.
     float f;   // the factor of the lane's part
     __device__ __forceinline__ void begin(float mi, float li, float mvi) {
-        const float top = fmaxf(m, warp_max(mi));
+        const float top = fmaxf(m, redux_max(mi));
         const float a = factor(m, top), b = factor(mi, top);
         l = l * a + warp_sum(li * b);
         m = top;
         float before = a;
         f = b;
         if (FP8) {
-            const float top_v = fmaxf(mv, warp_max(mvi));
+            const float top_v = fmaxf(mv, redux_max(mvi));
             before = factor(mv, top_v);
             f = factor(mvi, top_v);
             mv = top_v;
@@ -644,7 +651,7 @@ __device__ __forceinline__ void finish(const Params& p, const Joined<FP8>& j, in
             b[i] = bf16_round(r[i]);
             amax = fmaxf(amax, fabsf(b[i]));
         }
-        amax = warp_max(amax);
+        amax = redux_max(amax);
         const float scale = p.ue8m0 ? ue8m0_scale(amax) : group_scale(amax);
         const GroupDivider div(scale);
         if (live) {
@@ -715,57 +722,59 @@ decode_attention_kernel(const Params p) {
     const int blocks = min((int)gridDim.x, max(full * per_row, total / MIN_UNITS));
     if ((int)blockIdx.x >= blocks) return;
 
-    // ---- this block's range and this warp's share, each warp for itself
-    // The place of unit x: the threads whose rows end at x or before are
-    // counted, then the next one's rows walked. n: the units of its item.
-    auto locate = [&](int x, int& n) {
-        int ended = 0;
-#pragma unroll
-        for (int w = 0; w < WARPS; ++w)
-            ended += (earlier[w] + s_upto[32 * w + lane]) * per_row <= x;
-        ended = __reduce_add_sync(0xffffffffu, ended);
-        Place at = {x, ended * chunk, 0};
-        if (ended) {
-            at.before = s_upto[ended - 1];
-#pragma unroll
-            for (int w = 0; w < WARPS; ++w)
-                if ((ended - 1) >> 5 == w) at.before += earlier[w];
+    // ---- this block's range and this warp's share, each warp for itself: the
+    // places of its two cuts and of the warp's first unit. The threads whose
+    // rows end at x or before are counted, then the next one's rows walked.
+    const Cuts cuts(total, blocks);
+    int lo = 0, hi = total, end = total, n = 0;
+    Place at = {0, 0, 0};
+#pragma unroll 1
+    for (int c = 0; c < 3; ++c) {
+        if (c == 1 && (int)blockIdx.x + 1 == blocks) continue;
+        if (c == 2) {
+            const Cuts shares(hi - lo, WARPS);
+            end = lo + shares.at(warp + 1);
+            at.at = lo + shares.at(warp);
+            if (at.at == end) break;
+        } else {
+            at.at = cuts.at(blockIdx.x + c);
         }
+        int ended = 0, earlier = 0;
+#pragma unroll
+        for (int w = 0; w < WARPS; ++w) {
+            ended += (earlier + s_upto[32 * w + lane]) * per_row <= at.at;
+            earlier += s_scan[w];
+        }
+        ended = __reduce_add_sync(0xffffffffu, ended);
+        at.row = ended * chunk;
+        at.before = ended ? s_upto[ended - 1] : 0;
+#pragma unroll
+        for (int w = 0; w < WARPS - 1; ++w)
+            if (w < (ended - 1) >> 5) at.before += s_scan[w];
         for (;; ++at.row) {
             n = units_of(p, row_keys(p, at.row, false));
-            if (x < (at.before + n) * per_row) return at;
+            if (at.at < (at.before + n) * per_row) break;
             at.before += n;
         }
-    };
-    const Cuts cuts(total, blocks);
-    auto cut = [&](int i) {
-        if (i == blocks) return total;
-        const int x = cuts.at(i);
-        int n;
-        const Place at = locate(x, n);
-        const int s = at.before * per_row;
-        return settle(x, s + (x - s) / n * n, n);
-    };
-    const int lo = cut(blockIdx.x), hi = cut(blockIdx.x + 1);
-    const Cuts shares(hi - lo, WARPS);
+        if (c < 2) {
+            const int s = at.before * per_row;
+            (c ? hi : lo) = settle(at.at, s + (at.at - s) / n * n, n);
+        }
+    }
 
     // ---- this warp's range, an item after another
-    int at = lo + shares.at(warp);
-    const int end = lo + shares.at(warp + 1);
-    if (at < end) {
-        int n;
-        const Place begin = locate(at, n);
-        int row = begin.row, before = begin.before, keys = row_keys(p, row, false);
+    if (at.at < end) {
+        int keys = row_keys(p, at.row, false);
         for (;;) {
-            const int item = (at - before * per_row) / n;
-            const int s = before * per_row + item * n;
+            const int item = (at.at - at.before * per_row) / n;
+            const int s = at.before * per_row + item * n;
             const int stop = min(end, s + n);
             const int kvh = item / p.tiles, tile = item % p.tiles;
             const int head0 = kvh * p.group + tile * HEADS;
             const int heads = min(HEADS, p.group - tile * HEADS);
-            const int whole = 2 * (at == s) + (stop == s + n);
-            Slot<D>& slot = slots[2 * warp + (at == s)];
-            attend<D, FP8>(p, slot, row, kvh, head0, heads, (at - s) << p.unit_shift,
+            const int whole = 2 * (at.at == s) + (stop == s + n);
+            Slot<D>& slot = slots[2 * warp + (at.at == s)];
+            attend<D, FP8>(p, slot, at.row, kvh, head0, heads, (at.at - s) << p.unit_shift,
                            (int)min((int64_t)keys, (int64_t)(stop - s) << p.unit_shift), lane);
             __syncwarp();
             if (whole == 3) {
@@ -778,23 +787,23 @@ decode_attention_kernel(const Params p) {
                     j.mv = slot.mv[head];
 #pragma unroll
                     for (int e = 0; e < 4; ++e) j.acc[e] = slot.o[head][d4 + e];
-                    finish<D, FP8>(p, j, row, head0 + head, head < heads, d4);
+                    finish<D, FP8>(p, j, at.row, head0 + head, head < heads, d4);
                 }
             } else if (lane == 0) {
                 slot.start = s;
                 slot.n = n;
-                slot.row = row;
+                slot.row = at.row;
                 slot.head0 = head0;
                 slot.heads = heads;
                 slot.whole = whole;
             }
             __syncwarp();
-            at = stop;
-            if (at >= end) break;
-            while (at >= (before + n) * per_row) {
-                before += n;
-                ++row;
-                keys = row_keys(p, row, false);
+            at.at = stop;
+            if (stop >= end) break;
+            while (stop >= (at.before + n) * per_row) {
+                at.before += n;
+                ++at.row;
+                keys = row_keys(p, at.row, false);
                 n = units_of(p, keys);
             }
         }
@@ -878,7 +887,7 @@ decode_attention_kernel(const Params p) {
                 const float m = in ? __ldcg(&part.m[head]) : NEG_INF;
                 const float l = in ? __ldcg(&part.l[head]) : 0.0f;
                 const float mv = in ? __ldcg(&part.mv[head]) : NEG_INF;
-                constexpr int BATCH = 8;   // parts whose columns are in flight together
+                constexpr int BATCH = 16;   // parts whose columns are in flight together
                 float4 o[BATCH];
                 auto fetch = [&](int i) {
 #pragma unroll
