@@ -18,7 +18,10 @@ namespace {
 
 using namespace qb;
 
-constexpr int WARPS = 8;   // rows per block, one warp each
+constexpr int THREADS = 256;
+// A thread's pieces (8 elements of K and of V each) whose loads are in flight
+// together.
+constexpr int BATCH = 2;
 
 // 2^(b - 127); 0 is the subnormal 2^-127 and 255 NaN
 __device__ __forceinline__ float e8m0_float(uint32_t b) {
@@ -29,66 +32,87 @@ __device__ __forceinline__ float e8m0_float(uint32_t b) {
 // Quantises 8 values of a head held by LANES consecutive lanes (8 each).
 template <int LANES>
 __device__ __forceinline__ uint2 quant8(const uint4& raw, uint32_t& byte) {
-    float x[8];
-    bf16x8_to_float(raw, x);
-    // integer maximum of the magnitudes' bits: a NaN (above every infinity)
-    // is kept, which fmaxf would drop
-    uint32_t top = 0;
-#pragma unroll
-    for (int i = 0; i < 8; ++i) top = max(top, __float_as_uint(x[i]) & 0x7FFFFFFFu);
+    // the largest magnitude by its bits, two bf16 at a time; a NaN is above
+    // every infinity and so is kept
+    constexpr uint32_t ABS = 0x7FFF7FFFu;
+    uint32_t top = __vmaxu2(__vmaxu2(raw.x & ABS, raw.y & ABS),
+                            __vmaxu2(raw.z & ABS, raw.w & ABS));
 #pragma unroll
     for (int o = LANES / 2; o > 0; o >>= 1)
-        top = max(top, __shfl_xor_sync(0xffffffffu, top, o));
+        top = __vmaxu2(top, __shfl_xor_sync(0xffffffffu, top, o));
+    top = max(top << 16, top & 0xFFFF0000u);
     if (top >= 0x7F800000u) {
         byte = 255u;
         return make_uint2(0x7F7F7F7Fu, 0x7F7F7F7Fu);
     }
-    const float scale = ue8m0_scale(__uint_as_float(top));
-    byte = __float_as_uint(scale) >> 23;
-    const float inv = ue8m0_inverse(scale);
+    // ue8m0_scale's byte: the largest is f * 2^e with f in [1, 2), and f * 2^e
+    // <= 448 * 2^(e - 8) just when f <= 1.75; a bf16 f is 1.75 or differs from
+    // it by 2^-7 or more, so no quotient's rounding matters
+    top = max(top, __float_as_uint(1e-10f));
+    byte = (top >> 23) - 8u + ((top & 0x7FFFFFu) > 0x600000u);
+    const float inv = __uint_as_float((254u - byte) << 23);
+    const uint64_t by = f2pack(inv, inv);
+    const uint32_t w[4] = {raw.x, raw.y, raw.z, raw.w};
     uint32_t c[4];
 #pragma unroll
-    for (int i = 0; i < 4; ++i) c[i] = fp8x2(x[2 * i] * inv, x[2 * i + 1] * inv);
+    for (int i = 0; i < 4; ++i) {
+        const float2 x = bf16x2_float2(w[i]);
+        float a, b;
+        f2unpack(f2mul(f2pack(x.x, x.y), by), a, b);   // exact
+        c[i] = fp8x2(a, b);
+    }
     return make_uint2(c[0] | (c[1] << 16), c[2] | (c[3] << 16));
 }
 
+// A block takes `per_block` rows, each of `chunks` pieces for K and V; a
+// thread's pieces are THREADS apart, so LANES neighbouring lanes hold a head.
 template <int D>
-__global__ void __launch_bounds__(WARPS * 32)
+__global__ void __launch_bounds__(THREADS)
 kv_quant_write_kernel(const bf16* __restrict__ k, const bf16* __restrict__ v, int64_t k_ld,
                       int64_t v_ld, const int64_t* __restrict__ src,
                       const int64_t* __restrict__ dst, int64_t n, int64_t src_rows, int n_kv,
-                      uint8_t* __restrict__ k_codes, uint8_t* __restrict__ v_codes,
-                      uint8_t* __restrict__ k_scale, uint8_t* __restrict__ v_scale,
-                      int64_t pool_rows, uint32_t* status) {
-    constexpr int LANES = D / 8;   // lanes a head
-    const int lane = threadIdx.x & 31;
-    const int64_t i = (int64_t)blockIdx.x * WARPS + (threadIdx.x >> 5);
-    if (i >= n) return;
-    const int64_t d = dst[i], s = src ? src[i] : i;
-    if (d < 0) return;   // a row that is not kept
-    if (d >= pool_rows || s < 0 || s >= src_rows) {
-        if (lane == 0) atomicOr(status, STATUS_BAD_INDEX);
-        return;
-    }
-    const int chunks = n_kv * LANES;
-    for (int base = 0; base < chunks; base += 32) {
-        const int c = base + lane;
-        const bool in = c < chunks;
-        uint4 kr = make_uint4(0, 0, 0, 0), vr = kr;
-        if (in) {
-            kr = *reinterpret_cast<const uint4*>(k + s * k_ld + c * 8);
-            vr = *reinterpret_cast<const uint4*>(v + s * v_ld + c * 8);
+                      int chunks, int per_block, uint8_t* __restrict__ k_codes,
+                      uint8_t* __restrict__ v_codes, uint8_t* __restrict__ k_scale,
+                      uint8_t* __restrict__ v_scale, int64_t pool_rows, uint32_t* status) {
+    constexpr int LANES = D / 8;
+    const int64_t row0 = (int64_t)blockIdx.x * per_block;
+    const int all = (int)min((int64_t)per_block, n - row0) * chunks;
+    for (int base = threadIdx.x & ~31; base < all; base += THREADS * BATCH) {
+        uint4 raw[2][BATCH];
+        int64_t to[BATCH];   // the destination row, -1: none
+        int at[BATCH];
+#pragma unroll
+        for (int j = 0; j < BATCH; ++j) {
+            const int i = base + THREADS * j + (threadIdx.x & 31);
+            to[j] = -1;
+            raw[0][j] = raw[1][j] = make_uint4(0, 0, 0, 0);
+            if (i >= all) continue;
+            const int r = i / chunks;
+            at[j] = i - r * chunks;
+            const int64_t d = dst[row0 + r];
+            if (d < 0) continue;   // a row that is not kept
+            const int64_t s = src ? src[row0 + r] : row0 + r;
+            if (d >= pool_rows || s < 0 || s >= src_rows) {
+                if (at[j] == 0) atomicOr(status, STATUS_BAD_INDEX);
+                continue;
+            }
+            to[j] = d;
+            raw[0][j] = *reinterpret_cast<const uint4*>(k + s * k_ld + at[j] * 8);
+            raw[1][j] = *reinterpret_cast<const uint4*>(v + s * v_ld + at[j] * 8);
         }
-        uint32_t kb, vb;
-        const uint2 kq = quant8<LANES>(kr, kb);
-        const uint2 vq = quant8<LANES>(vr, vb);
-        if (in) {
-            const int64_t at = d * n_kv * D + c * 8;
-            *reinterpret_cast<uint2*>(k_codes + at) = kq;
-            *reinterpret_cast<uint2*>(v_codes + at) = vq;
-            if (c % LANES == 0) {
-                k_scale[d * n_kv + c / LANES] = (uint8_t)kb;
-                v_scale[d * n_kv + c / LANES] = (uint8_t)vb;
+#pragma unroll
+        for (int j = 0; j < BATCH; ++j) {
+            if (base + THREADS * j >= all) break;   // (the same for a warp)
+            uint32_t kb, vb;
+            const uint2 kq = quant8<LANES>(raw[0][j], kb);
+            const uint2 vq = quant8<LANES>(raw[1][j], vb);
+            if (to[j] < 0) continue;
+            const int64_t place = to[j] * n_kv * D + at[j] * 8;
+            *reinterpret_cast<uint2*>(k_codes + place) = kq;
+            *reinterpret_cast<uint2*>(v_codes + place) = vq;
+            if (at[j] % LANES == 0) {
+                k_scale[to[j] * n_kv + at[j] / LANES] = (uint8_t)kb;
+                v_scale[to[j] * n_kv + at[j] / LANES] = (uint8_t)vb;
             }
         }
     }
@@ -105,38 +129,64 @@ __device__ __forceinline__ uint4 dequant8(const uint2& codes, float scale) {
 }
 
 template <int D>
-__global__ void __launch_bounds__(WARPS * 32)
+__global__ void __launch_bounds__(THREADS)
 kv_quant_read_kernel(const uint8_t* __restrict__ k_codes, const uint8_t* __restrict__ v_codes,
                      const uint8_t* __restrict__ k_scale, const uint8_t* __restrict__ v_scale,
                      int64_t pool_rows, const int64_t* __restrict__ src,
-                     const int64_t* __restrict__ dst, int64_t n, int n_kv, bf16* __restrict__ k,
-                     bf16* __restrict__ v, int64_t k_ld, int64_t v_ld, int64_t out_rows,
-                     uint32_t* status) {
+                     const int64_t* __restrict__ dst, int64_t n, int n_kv, int chunks,
+                     int per_block, bf16* __restrict__ k, bf16* __restrict__ v, int64_t k_ld,
+                     int64_t v_ld, int64_t out_rows, uint32_t* status) {
     constexpr int LANES = D / 8;
-    const int lane = threadIdx.x & 31;
-    const int64_t i = (int64_t)blockIdx.x * WARPS + (threadIdx.x >> 5);
-    if (i >= n) return;
-    const int64_t s = src[i], d = dst ? dst[i] : i;
-    if (d < 0) return;
-    if (d >= out_rows) {
-        if (lane == 0) atomicOr(status, STATUS_BAD_INDEX);
-        return;
-    }
-    const bool bad = s < 0 || s >= pool_rows;   // flagged, and zeros written
-    if (bad && lane == 0) atomicOr(status, STATUS_BAD_INDEX);
-    const int chunks = n_kv * LANES;
-    for (int c = lane; c < chunks; c += 32) {
-        uint4 ko = make_uint4(0, 0, 0, 0), vo = ko;
-        if (!bad) {
-            const int64_t at = s * n_kv * D + c * 8, head = s * n_kv + c / LANES;
-            ko = dequant8(*reinterpret_cast<const uint2*>(k_codes + at),
-                          e8m0_float(k_scale[head]));
-            vo = dequant8(*reinterpret_cast<const uint2*>(v_codes + at),
-                          e8m0_float(v_scale[head]));
+    const int64_t row0 = (int64_t)blockIdx.x * per_block;
+    const int all = (int)min((int64_t)per_block, n - row0) * chunks;
+    for (int base = threadIdx.x; base < all; base += THREADS * BATCH) {
+        uint2 codes[2][BATCH];
+        uint32_t bytes[2][BATCH];
+        int64_t to[BATCH];   // the output row, -1: none
+        int at[BATCH];
+#pragma unroll
+        for (int j = 0; j < BATCH; ++j) {
+            const int i = base + THREADS * j;
+            to[j] = -1;
+            codes[0][j] = codes[1][j] = make_uint2(0, 0);
+            bytes[0][j] = bytes[1][j] = 127u;
+            if (i >= all) continue;
+            const int r = i / chunks;
+            at[j] = i - r * chunks;
+            const int64_t d = dst ? dst[row0 + r] : row0 + r;
+            if (d < 0) continue;
+            const int64_t s = src[row0 + r];
+            if (d >= out_rows || s < 0 || s >= pool_rows) {
+                if (at[j] == 0) atomicOr(status, STATUS_BAD_INDEX);
+                to[j] = d < out_rows ? d : -1;   // zeros for a bad source
+                continue;
+            }
+            to[j] = d;
+            const int64_t place = s * n_kv * D + at[j] * 8, head = s * n_kv + at[j] / LANES;
+            codes[0][j] = *reinterpret_cast<const uint2*>(k_codes + place);
+            codes[1][j] = *reinterpret_cast<const uint2*>(v_codes + place);
+            bytes[0][j] = k_scale[head];
+            bytes[1][j] = v_scale[head];
         }
-        *reinterpret_cast<uint4*>(k + d * k_ld + c * 8) = ko;
-        *reinterpret_cast<uint4*>(v + d * v_ld + c * 8) = vo;
+#pragma unroll
+        for (int j = 0; j < BATCH; ++j) {
+            if (to[j] < 0) continue;
+            *reinterpret_cast<uint4*>(k + to[j] * k_ld + at[j] * 8) =
+                dequant8(codes[0][j], e8m0_float(bytes[0][j]));
+            *reinterpret_cast<uint4*>(v + to[j] * v_ld + at[j] * 8) =
+                dequant8(codes[1][j], e8m0_float(bytes[1][j]));
+        }
     }
+}
+
+// Rows of a block: pieces for each thread's batches, but a block for at least
+// one row, and (so that few rows still spread over the GPU) no more rows than
+// leave about two blocks an SM.
+int rows_per_block(int64_t n, int chunks) {
+    const int64_t most = THREADS * BATCH * 2 / chunks;
+    const int64_t spread = n / 296;
+    const int64_t rows = most < spread ? most : spread;
+    return rows < 1 ? 1 : (int)rows;
 }
 
 int check_cache(const char* who, int64_t n, int n_kv, int head_dim, int64_t k_ld, int64_t v_ld,
@@ -182,11 +232,12 @@ extern "C" int qb_kv_quant_write(const void* k, const void* v, int64_t k_ld, int
     if (n == 0) return QB_OK;
     uint32_t* status = device_status_ptr();
     if (!status) return launch_status("qb_kv_quant_write: status word");
-    const unsigned blocks = (unsigned)((n + WARPS - 1) / WARPS);
+    const int chunks = n_kv * (head_dim / 8), per_block = rows_per_block(n, chunks);
+    const unsigned blocks = (unsigned)((n + per_block - 1) / per_block);
     auto* kernel = head_dim == 128 ? kv_quant_write_kernel<128> : kv_quant_write_kernel<64>;
-    kernel<<<blocks, WARPS * 32, 0, (cudaStream_t)stream>>>(
+    kernel<<<blocks, THREADS, 0, (cudaStream_t)stream>>>(
         (const bf16*)k, (const bf16*)v, k_ld, v_ld, src, dst, n, src_rows, n_kv,
-        (uint8_t*)k_codes, (uint8_t*)v_codes, k_scale, v_scale, pool_rows, status);
+        chunks, per_block, (uint8_t*)k_codes, (uint8_t*)v_codes, k_scale, v_scale, pool_rows, status);
     return launch_status(who);
 }
 
@@ -204,10 +255,11 @@ extern "C" int qb_kv_quant_read(const void* k_codes, const void* v_codes, const 
     if (n == 0) return QB_OK;
     uint32_t* status = device_status_ptr();
     if (!status) return launch_status("qb_kv_quant_read: status word");
-    const unsigned blocks = (unsigned)((n + WARPS - 1) / WARPS);
+    const int chunks = n_kv * (head_dim / 8), per_block = rows_per_block(n, chunks);
+    const unsigned blocks = (unsigned)((n + per_block - 1) / per_block);
     auto* kernel = head_dim == 128 ? kv_quant_read_kernel<128> : kv_quant_read_kernel<64>;
-    kernel<<<blocks, WARPS * 32, 0, (cudaStream_t)stream>>>(
+    kernel<<<blocks, THREADS, 0, (cudaStream_t)stream>>>(
         (const uint8_t*)k_codes, (const uint8_t*)v_codes, k_scale, v_scale, pool_rows, src, dst,
-        n, n_kv, (bf16*)k, (bf16*)v, k_ld, v_ld, out_rows, status);
+        n, n_kv, chunks, per_block, (bf16*)k, (bf16*)v, k_ld, v_ld, out_rows, status);
     return launch_status(who);
 }
