@@ -7,8 +7,14 @@
 // e^{x_bv}. Within a beam that order is the order of the logits, so each beam
 // offers its n_out largest logits (equal ones: lowest token first) before
 // lse_b is known, and the group's n_out best offers win (equal scores: lowest
-// beam first, then the beam's own order). HBM-bound: the logits are to be read
-// once; sums are kept in fp32.
+// beam first, then the beam's own order). HBM-bound: the logits are read once,
+// each block a run of one beam's; a logit costs a maximum, an exponential and
+// an addition in fp32. A block keeps its n_out best so far as sorted keys
+// (value, lower token first) and looks at single logits only where a thread's
+// largest of the current tile passes the least of them; the threads that have
+// one put it forward together, and again, until none passes. The block that
+// completes its group (a counter) joins the runs and the beams, in an order
+// that does not depend on who came last.
 #include "common.cuh"
 
 namespace {
@@ -17,7 +23,12 @@ using namespace qb;
 
 constexpr int MAX_BEAMS = 32;
 constexpr int MAX_OUT = 32;
-constexpr int SELECT_THREADS = 512;
+constexpr int MAX_ROWS = 65535;        // groups * beams
+constexpr int THREADS = 256;
+constexpr int PER_THREAD = 16;         // logits of a thread in a tile
+constexpr int TILE = THREADS * PER_THREAD;
+constexpr int JOIN_BYTES = 40 * 1024;  // a group's keys in the join
+constexpr float LOG2E = 1.44269504088896341f;
 
 // A logit as an unsigned key in the order of the values; NaN is taken as -inf
 __device__ __forceinline__ uint32_t order_key(float x) {
@@ -25,105 +36,314 @@ __device__ __forceinline__ uint32_t order_key(float x) {
     const uint32_t b = __float_as_uint(x == 0.0f ? 0.0f : x);   // -0 equals 0
     return b ^ ((uint32_t)((int32_t)b >> 31) | 0x80000000u);
 }
-__device__ __forceinline__ float key_value(uint32_t k) {
+__device__ __forceinline__ float key_value(uint64_t key) {
+    const uint32_t k = (uint32_t)(key >> 32);
     return __uint_as_float(k & 0x80000000u ? k ^ 0x80000000u : ~k);
 }
-// (value, lower index first) as one key; distinct for distinct indexes
+// (value, lower index first) as one key; distinct for distinct indexes, and
+// above every number under 2^32
 __device__ __forceinline__ uint64_t offer_key(float x, uint32_t index) {
     return ((uint64_t)order_key(x) << 32) | (0xFFFFFFFFu - index);
 }
+__device__ __forceinline__ uint32_t key_index(uint64_t key) { return 0xFFFFFFFFu - (uint32_t)key; }
 
 __device__ __forceinline__ uint64_t warp_max64(uint64_t v) {
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) {
-        const uint64_t u = __shfl_xor_sync(0xffffffffu, v, o);
-        v = u > v ? u : v;
-    }
-    return v;
+    const uint32_t hi = __reduce_max_sync(0xffffffffu, (uint32_t)(v >> 32));
+    const uint32_t lo =
+        __reduce_max_sync(0xffffffffu, (uint32_t)(v >> 32) == hi ? (uint32_t)v : 0u);
+    return ((uint64_t)hi << 32) | lo;
 }
 
+// the largest of a warp's values (none is NaN)
+__device__ __forceinline__ float redux_max(float x) {
+    float r;
+    asm("redux.sync.max.f32 %0, %1, 0xffffffff;" : "=f"(r) : "f"(x));
+    return r;
+}
+
+__device__ __forceinline__ float exp_approx(float x) {
+    float r;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x * LOG2E));
+    return r;
+}
+
+// A 16-byte vector of logits as floats
 template <typename T>
-__device__ __forceinline__ float logit(const T* row, int64_t i);
-template <>
-__device__ __forceinline__ float logit<float>(const float* row, int64_t i) { return row[i]; }
-template <>
-__device__ __forceinline__ float logit<bf16>(const bf16* row, int64_t i) {
+constexpr int PER_VECTOR = 16 / sizeof(T);
+__device__ __forceinline__ void unpack(const uint4& v, float (&x)[4]) {
+    x[0] = __uint_as_float(v.x);
+    x[1] = __uint_as_float(v.y);
+    x[2] = __uint_as_float(v.z);
+    x[3] = __uint_as_float(v.w);
+}
+__device__ __forceinline__ void unpack(const uint4& v, float (&x)[8]) { bf16x8_to_float(v, x); }
+__device__ __forceinline__ float logit(const float* row, int64_t i) { return row[i]; }
+__device__ __forceinline__ float logit(const bf16* row, int64_t i) {
     return __bfloat162float(row[i]);
 }
 
-// One block a beam: the row's lse and its n_out largest logits as keys.
+struct SelectParams {
+    const void* logits;
+    int64_t ld, vocab;
+    int beams, n_out, splits;
+    const float* scores;
+    const uint8_t* finished;
+    int64_t pad;
+    uint32_t* arrived;     // a counter a group, zero between launches
+    uint64_t* keys;        // [rows, splits, n_out]
+    float2* sums;          // [rows, splits]: the largest logit, sum e^(x - largest)
+    float* scores_out;
+    int32_t* parent_out;
+    int64_t* token_out;
+};
+
+// Block (split, row): a run of one beam's logits.
 template <typename T>
-__global__ void __launch_bounds__(SELECT_THREADS)
-beam_offers_kernel(const T* __restrict__ logits, int64_t ld, int64_t vocab,
-                   const uint8_t* __restrict__ finished, int n_out, float* __restrict__ lse_out,
-                   uint64_t* __restrict__ offers) {
-    __shared__ uint64_t s_key[SELECT_THREADS / 32];
-    __shared__ float scratch[32];
-    const int64_t b = blockIdx.x;
-    if (finished && finished[b]) return;
-    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-    const T* row = logits + b * ld;
-    uint64_t below = ~0ull;
-    float m = -INFINITY;
-    for (int r = 0; r < n_out; ++r) {
-        uint64_t best = 0;
-        for (int64_t i = threadIdx.x; i < vocab; i += SELECT_THREADS) {
-            const uint64_t k = offer_key(logit(row, i), (uint32_t)i);
-            if (k < below && k > best) best = k;
+__global__ void __launch_bounds__(THREADS)
+beam_select_kernel(const SelectParams p) {
+    constexpr int VE = PER_VECTOR<T>, VECTORS = PER_THREAD / VE;
+    __shared__ uint64_t s_key[MAX_OUT + THREADS];   // the best so far, in order; then new ones
+    __shared__ uint32_t s_new, s_group[32];
+    __shared__ float s_m[THREADS / 32], s_s[THREADS / 32];
+    __shared__ bool s_last;
+    __shared__ float s_lse[MAX_BEAMS];
+    extern __shared__ uint64_t s_lists[];           // the join's: [beams, splits, n_out]
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+    const int64_t row = blockIdx.y, group = row / p.beams;
+    const int split = blockIdx.x, n_out = p.n_out;
+
+    if (!p.finished || !p.finished[row]) {
+        const T* x_row = (const T*)p.logits + row * p.ld;
+        // single logits up to the first 16-byte boundary, vectors, single ones
+        const int off = (int)((uintptr_t)x_row / sizeof(T) % VE);
+        const int head = (int)min(p.vocab, (int64_t)(off ? VE - off : 0));
+        const int64_t vectors = (p.vocab - head) / VE;
+        const int tail = (int)(p.vocab - head - vectors * VE);
+        int single = -1;   // this thread's one, in the first tile
+        if (split == 0 && tid < head) single = tid;
+        if (split == p.splits - 1 && tid >= 32 && tid - 32 < tail)
+            single = (int)(p.vocab - tail) + tid - 32;
+        const uint4* body = reinterpret_cast<const uint4*>(x_row + head);
+        const int v1 = (int)(vectors * (split + 1) / p.splits);
+        int v = (int)(vectors * split / p.splits) + tid;
+
+        if (tid < n_out) s_key[tid] = n_out - tid;   // under every offer
+        if (tid == 0) s_new = 0;
+        uint64_t least = 0;
+        float m = -INFINITY, sum = 0.0f;
+        const float x_single = single >= 0 ? logit(x_row, single) : -INFINITY;
+        uint4 raw[VECTORS];
+#pragma unroll
+        for (int i = 0; i < VECTORS; ++i) {
+            raw[i] = make_uint4(0, 0, 0, 0);
+            if (v + i * THREADS < v1) raw[i] = __ldcs(body + v + i * THREADS);
         }
-        best = warp_max64(best);
+        for (bool first = true;; first = false) {
+            float x[VECTORS][VE];
+#pragma unroll
+            for (int i = 0; i < VECTORS; ++i) {
+                unpack(raw[i], x[i]);
+                if (v + i * THREADS >= v1)
+#pragma unroll
+                    for (int e = 0; e < VE; ++e) x[i][e] = -INFINITY;
+            }
+            const int at = v;
+            v += VECTORS * THREADS;
+            const bool more = v - tid < v1;   // (the same for the block)
+#pragma unroll
+            for (int i = 0; i < VECTORS; ++i)
+                if (v + i * THREADS < v1) raw[i] = __ldcs(body + v + i * THREADS);
+
+            // the sum, against the largest so far
+            float top = first ? x_single : -INFINITY;
+            if (top != top) top = -INFINITY;
+#pragma unroll
+            for (int i = 0; i < VECTORS; ++i)
+#pragma unroll
+                for (int e = 0; e < VE; ++e) top = fmaxf(top, x[i][e]);
+            if (top > m) {
+                sum *= exp_approx(m - top);
+                m = top;
+            }
+            const float ref = m > -INFINITY ? m : 0.0f;
+            if (first && single >= 0) sum += exp_approx(x_single - ref);
+            float part = 0.0f;
+#pragma unroll
+            for (int i = 0; i < VECTORS; ++i)
+#pragma unroll
+                for (int e = 0; e < VE; ++e) part += exp_approx(x[i][e] - ref);
+            sum += part;
+
+            // the thread's best key under `limit`
+            auto best_under = [&](uint64_t limit) {
+                uint64_t best = 0;
+#pragma unroll
+                for (int i = 0; i < VECTORS; ++i)
+#pragma unroll
+                    for (int e = 0; e < VE; ++e) {
+                        const uint64_t k =
+                            offer_key(x[i][e], head + (uint32_t)(at + i * THREADS) * VE + e);
+                        if (at + i * THREADS < v1 && k < limit && k > best) best = k;
+                    }
+                if (first && single >= 0) {
+                    const uint64_t k = offer_key(x_single, single);
+                    if (k < limit && k > best) best = k;
+                }
+                return best;
+            };
+            if (first) {
+                // n_out groups of threads or more: that many logits reach the
+                // least of their maxima, so nothing under it can be chosen
+                const bool some = at < v1 || single >= 0;
+                const uint32_t mine = some ? order_key(top) : 0u;
+                if (n_out <= THREADS / 32) {
+                    const uint32_t g = __reduce_max_sync(0xffffffffu, mine);
+                    if (lane == 0) s_group[warp] = g;
+                } else {
+                    const uint32_t g = __reduce_max_sync(0xFFu << (lane & 24), mine);
+                    if (lane % 8 == 0) s_group[tid / 8] = g;
+                }
+                __syncthreads();
+                const int groups = n_out <= THREADS / 32 ? THREADS / 32 : 32;
+                const uint32_t g =
+                    __reduce_min_sync(0xffffffffu, lane < groups ? s_group[lane] : ~0u);
+                least = g ? ((uint64_t)g << 32) - 1 : 0;   // (0: a group has no logit)
+            }
+            uint64_t key = order_key(top) >= (uint32_t)(least >> 32) ? best_under(~0ull) : 0;
+            for (;;) {
+                const bool put = key > least;
+                const int fresh = __syncthreads_count(put);
+                if (fresh == 0) break;
+                if (put) {
+                    s_key[n_out + atomicAdd(&s_new, 1u)] = key;
+                    key = best_under(key);
+                }
+                __syncthreads();
+                // the places of the n_out best; a key's place is the number
+                // above it, so the order of arrival does not matter
+                const int n = n_out + fresh;
+                uint64_t mine[2];
+                int place[2];
+#pragma unroll
+                for (int c = 0; c < 2; ++c) {
+                    place[c] = n_out;
+                    if (tid + c * THREADS >= n) continue;
+                    mine[c] = s_key[tid + c * THREADS];
+                    int above = 0;
+                    for (int j = 0; j < n; ++j) above += s_key[j] > mine[c];
+                    place[c] = above;
+                }
+                __syncthreads();
+#pragma unroll
+                for (int c = 0; c < 2; ++c)
+                    if (place[c] < n_out) s_key[place[c]] = mine[c];
+                if (tid == 0) s_new = 0;
+                __syncthreads();
+                least = s_key[n_out - 1];
+            }
+            if (!more) break;
+        }
+        // ---- the run's results
+        const float top = redux_max(m);
+        const float s = warp_sum(m > -INFINITY ? sum * exp_approx(m - top) : sum);
+        if (lane == 0) {
+            s_m[warp] = top;
+            s_s[warp] = s;
+        }
+        const int64_t at = row * p.splits + split;
+        if (tid < n_out) __stcg(p.keys + at * n_out + tid, s_key[tid]);
         __syncthreads();
-        if (lane == 0) s_key[warp] = best;
-        __syncthreads();
-        for (int w = 0; w < SELECT_THREADS / 32; ++w) best = s_key[w] > best ? s_key[w] : best;
-        below = best;
-        if (r == 0) m = key_value((uint32_t)(best >> 32));
-        if (threadIdx.x == 0) offers[b * n_out + r] = best;
+        if (tid == 0) {
+            float all = s_m[0];
+            for (int w = 1; w < THREADS / 32; ++w) all = fmaxf(all, s_m[w]);
+            float t = 0.0f;
+            for (int w = 0; w < THREADS / 32; ++w)
+                t += s_m[w] > -INFINITY ? s_s[w] * exp_approx(s_m[w] - all) : s_s[w];
+            __stcg(p.sums + at, make_float2(all, t));
+        }
     }
-    float sum = 0.0f;
-    const float ref = m > -INFINITY ? m : 0.0f;
-    for (int64_t i = threadIdx.x; i < vocab; i += SELECT_THREADS) sum += expf(logit(row, i) - ref);
-    sum = block_sum(sum, scratch);
-    if (threadIdx.x == 0) lse_out[b] = m + logf(sum);
+    // ---- the group's last block joins
+    __syncthreads();
+    if (tid == 0) {
+        __threadfence();
+        const uint32_t all = (uint32_t)(p.beams * p.splits);
+        s_last = atomicAdd(p.arrived + group, 1u) == all - 1;
+        if (s_last) p.arrived[group] = 0;   // for the next launch
+        __threadfence();
+    }
+    __syncthreads();
+    if (!s_last) return;
+    const int64_t row0 = group * p.beams;
+    const int list = p.splits * n_out;
+    for (int i = tid; i < p.beams * list; i += THREADS)
+        s_lists[i] = __ldcg(p.keys + row0 * list + i);
+    __syncthreads();
+    for (int b = warp; b < p.beams; b += THREADS / 32) {
+        if (p.finished && p.finished[row0 + b]) continue;
+        // lse, then the beam's offers in order, over its first run's keys
+        float m = -INFINITY;
+        for (int i = lane; i < p.splits; i += 32)
+            m = fmaxf(m, __ldcg(p.sums + (row0 + b) * p.splits + i).x);
+        m = redux_max(m);
+        float sum = 0.0f;
+        for (int i = lane; i < p.splits; i += 32) {
+            const float2 part = __ldcg(p.sums + (row0 + b) * p.splits + i);
+            sum += part.x > -INFINITY ? part.y * exp_approx(part.x - m) : part.y;
+        }
+        sum = warp_sum(sum);
+        if (lane == 0) s_lse[b] = m + logf(sum);
+        if (p.splits > 1) {
+            uint64_t* keys = s_lists + b * list;
+            uint64_t limit = ~0ull, chosen = 0;   // of rank `lane`
+            for (int r = 0; r < n_out; ++r) {
+                uint64_t best = 0;
+                for (int i = lane; i < list; i += 32) {
+                    const uint64_t k = keys[i];
+                    if (k < limit && k > best) best = k;
+                }
+                limit = warp_max64(best);
+                if (lane == r) chosen = limit;
+            }
+            __syncwarp();
+            if (lane < n_out) keys[lane] = chosen;
+        }
+    }
+    __syncthreads();
+    if (warp != 0) return;
+    // a beam a lane: its next offer
+    const bool live = lane < p.beams;
+    const bool done = live && p.finished && p.finished[row0 + lane];
+    const float score = live ? p.scores[row0 + lane] : 0.0f;
+    int rank = 0;
+    auto offer = [&]() -> uint64_t {
+        if (!live || rank == n_out) return 0;
+        float s = rank ? -INFINITY : score;
+        if (!done) s = score + (key_value(s_lists[lane * list + rank]) - s_lse[lane]);
+        return offer_key(s, lane * n_out + rank);
+    };
+    uint64_t mine = offer();
+    for (int r = 0; r < n_out; ++r) {
+        const uint64_t best = warp_max64(mine);
+        if (mine == best) {   // (one lane: keys differ)
+            const int64_t at = group * n_out + r;
+            p.scores_out[at] = key_value(best);
+            p.parent_out[at] = lane;
+            p.token_out[at] = done ? p.pad : (int64_t)key_index(s_lists[lane * list + rank]);
+            ++rank;
+            mine = offer();
+        }
+    }
 }
 
-// One warp a group: the n_out best of its beams' offers.
-__global__ void beam_join_kernel(const float* __restrict__ lse, const uint64_t* __restrict__ offers,
-                                 const float* __restrict__ scores,
-                                 const uint8_t* __restrict__ finished, int beams, int64_t pad,
-                                 int n_out, float* __restrict__ scores_out,
-                                 int32_t* __restrict__ parent_out,
-                                 int64_t* __restrict__ token_out) {
-    const int64_t group = blockIdx.x;
-    const int lane = threadIdx.x;
-    uint64_t below = ~0ull;
-    for (int r = 0; r < n_out; ++r) {
-        uint64_t best = 0;
-        for (int c = lane; c < beams * n_out; c += 32) {
-            const int64_t b = group * beams + c / n_out;
-            const int rank = c % n_out;
-            float s;
-            if (finished && finished[b]) {
-                s = rank == 0 ? scores[b] : -INFINITY;
-            } else {
-                const float x = key_value((uint32_t)(offers[b * n_out + rank] >> 32));
-                s = scores[b] + (x - lse[b]);
-            }
-            const uint64_t k = offer_key(s, (uint32_t)c);
-            if (k < below && k > best) best = k;
-        }
-        best = warp_max64(best);
-        below = best;
-        if (lane == 0) {
-            const int c = (int)(0xFFFFFFFFu - (uint32_t)best);
-            const int64_t b = group * beams + c / n_out, at = group * n_out + r;
-            scores_out[at] = key_value((uint32_t)(best >> 32));
-            parent_out[at] = c / n_out;
-            token_out[at] = finished && finished[b]
-                                ? pad
-                                : (int64_t)(0xFFFFFFFFu - (uint32_t)offers[b * n_out + c % n_out]);
-        }
-    }
+// Runs that a beam's logits are cut into: about five blocks an SM, no run
+// under a tile, and the group's keys in the join's shared memory.
+int select_splits(int64_t rows, int beams, int64_t vocab, int n_out) {
+    const int64_t tiles = (vocab + TILE - 1) / TILE;
+    int64_t splits = 740 / rows;
+    splits = splits < tiles ? splits : tiles;
+    const int64_t most = JOIN_BYTES / 8 / ((int64_t)beams * n_out);
+    splits = splits < most ? splits : most;
+    return splits < 1 ? 1 : (int)splits;
 }
 
 // ---- reordering -------------------------------------------------------------
@@ -220,10 +440,15 @@ beam_reorder_kernel(const int32_t* __restrict__ parents, const int32_t* __restri
 
 extern "C" int qb_beam_select_workspace(int64_t groups, int beams, int64_t vocab, int n_out,
                                         int64_t* bytes) {
-    if (!bytes || groups < 0 || beams <= 0 || beams > MAX_BEAMS || n_out <= 0 ||
-        n_out > MAX_OUT || vocab < n_out || vocab > 0x7fffffffLL)
+    if (!bytes || groups < 0 || beams <= 0 || beams > MAX_BEAMS || groups > MAX_ROWS ||
+        groups * beams > MAX_ROWS || n_out <= 0 || n_out > MAX_OUT || vocab < n_out ||
+        vocab > 0x7fffffffLL)
         return invalid("qb_beam_select_workspace: bad sizes");
-    *bytes = groups * beams * ((int64_t)n_out * 8 + 8);
+    // the counters, always at the same place, then the runs' keys and sums
+    *bytes = MAX_ROWS * 4 + 4;
+    if (groups)
+        *bytes += groups * beams * select_splits(groups * beams, beams, vocab, n_out) *
+                  ((int64_t)n_out * 8 + 8);
     return QB_OK;
 }
 
@@ -235,28 +460,43 @@ extern "C" int qb_beam_select(const void* logits, int logits_bf16, int64_t logit
     const char* who = "qb_beam_select";
     if (beams <= 0 || beams > MAX_BEAMS || n_out <= 0 || n_out > MAX_OUT)
         return invalid("qb_beam_select: 1 to 32 beams and 1 to 32 outputs a group");
-    if (groups < 0 || groups * beams > 0x7fffffffLL || vocab < n_out || vocab > 0x7fffffffLL ||
-        logits_ld < vocab)
-        return invalid("qb_beam_select: vocab must hold n_out tokens and logits_ld the vocab");
+    if (groups < 0 || groups > MAX_ROWS || groups * beams > MAX_ROWS || vocab < n_out ||
+        vocab > 0x7fffffffLL || logits_ld < vocab)
+        return invalid("qb_beam_select: at most 65,535 rows, vocab must hold n_out tokens and "
+                       "logits_ld the vocab");
     if (groups == 0) return QB_OK;
     if (!logits || !scores || !scores_out || !parent_out || !token_out)
         return invalid("qb_beam_select: NULL tensor");
+    if (!aligned(logits, logits_bf16 ? 2 : 4))
+        return invalid("qb_beam_select: logits are not aligned to their type");
     int64_t need = 0;
     const int st = qb_beam_select_workspace(groups, beams, vocab, n_out, &need);
     if (st) return st;
     if (!workspace || workspace_bytes < need || !aligned(workspace, 16))
         return invalid("qb_beam_select: the workspace is too small (qb_beam_select_workspace)");
-    uint64_t* offers = (uint64_t*)workspace;
-    float* lse = (float*)(offers + groups * beams * n_out);
-    const unsigned rows = (unsigned)(groups * beams);
+    const int64_t rows = groups * beams;
+    SelectParams p;
+    p.logits = logits;
+    p.ld = logits_ld;
+    p.vocab = vocab;
+    p.beams = beams;
+    p.n_out = n_out;
+    p.splits = select_splits(rows, beams, vocab, n_out);
+    p.scores = scores;
+    p.finished = finished;
+    p.pad = pad;
+    p.arrived = (uint32_t*)workspace;
+    p.keys = (uint64_t*)((char*)workspace + MAX_ROWS * 4 + 4);
+    p.sums = (float2*)(p.keys + rows * p.splits * n_out);
+    p.scores_out = scores_out;
+    p.parent_out = parent_out;
+    p.token_out = token_out;
+    const dim3 grid((unsigned)p.splits, (unsigned)rows);
+    const int bytes = beams * p.splits * n_out * 8;
     if (logits_bf16)
-        beam_offers_kernel<bf16><<<rows, SELECT_THREADS, 0, (cudaStream_t)stream>>>(
-            (const bf16*)logits, logits_ld, vocab, finished, n_out, lse, offers);
+        beam_select_kernel<bf16><<<grid, THREADS, bytes, (cudaStream_t)stream>>>(p);
     else
-        beam_offers_kernel<float><<<rows, SELECT_THREADS, 0, (cudaStream_t)stream>>>(
-            (const float*)logits, logits_ld, vocab, finished, n_out, lse, offers);
-    beam_join_kernel<<<(unsigned)groups, 32, 0, (cudaStream_t)stream>>>(
-        lse, offers, scores, finished, beams, pad, n_out, scores_out, parent_out, token_out);
+        beam_select_kernel<float><<<grid, THREADS, bytes, (cudaStream_t)stream>>>(p);
     return launch_status(who);
 }
 

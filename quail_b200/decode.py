@@ -171,31 +171,58 @@ def kv_quant_read(kv: QuantLayer, src, dst=None, out=None):
     return k, v
 
 
-_workspaces = {}   # (device, stream) -> the attention's workspace there
+_workspaces = {}   # (use, device, stream) -> a workspace
+
+
+def _stream_workspace(use, device, need):
+    """The current stream's own zeroed workspace of `need` bytes or more, kept
+    (each call leaves its counters zero). A graph that is being captured must
+    not share it (the graph may be replayed beside the stream), so there a call
+    gets a fresh one, whose zeroing the graph repeats: pass workspace= to spare
+    that."""
+    key = use, device, torch._C._cuda_getCurrentRawStream(device)
+    held = _workspaces.get(key)
+    if held is not None and held.shape[0] >= need and (
+            not torch.cuda.is_current_stream_capturing()):
+        return held
+    held = torch.zeros(need, dtype=torch.uint8, device=torch.device("cuda", device))
+    if not torch.cuda.is_current_stream_capturing():
+        _workspaces[key] = held
+    return held
+
+
+_attention_bytes = {}   # device -> bytes
+
+
+def _decode_bytes(device):
+    need = _attention_bytes.get(device)
+    if need is None:
+        out = ctypes.c_int64(0)
+        with torch.cuda.device(device):
+            nat.call("qb_decode_attention_workspace", ctypes.byref(out))
+        need = _attention_bytes[device] = out.value
+    return need
 
 
 def decode_workspace(device="cuda"):
     """A workspace for decode_attention calls that follow one another (one
     stream, one captured graph): its size does not depend on a call's, and each
     call leaves it as it found it."""
-    with torch.cuda.device(device):
-        need = ctypes.c_int64(0)
-        nat.call("qb_decode_attention_workspace", ctypes.byref(need))
-        return torch.zeros(need.value, dtype=torch.uint8, device="cuda")
+    index = torch.empty(0, device=device).get_device()
+    return torch.zeros(_decode_bytes(index), dtype=torch.uint8, device=device)
 
 
-def _stream_workspace(device):
-    """The current stream's own workspace, kept. A graph that is being captured
-    must not share it (the graph may be replayed beside the stream), so there a
-    call gets a fresh one, whose zeroing the graph repeats: pass workspace= to
-    spare that."""
-    if torch.cuda.is_current_stream_capturing():
-        return decode_workspace(device)
-    stream = torch._C._cuda_getCurrentRawStream(device)
-    held = _workspaces.get((device, stream))
-    if held is None:
-        held = _workspaces[device, stream] = decode_workspace(device)
-    return held
+def _select_bytes(groups, beams, vocab, n_out):
+    need = ctypes.c_int64(0)
+    nat.call("qb_beam_select_workspace", groups, beams, vocab, n_out, ctypes.byref(need))
+    return need.value
+
+
+def beam_workspace(groups, beams, vocab, n_out=None, device="cuda"):
+    """A workspace for beam_select calls of these sizes that follow one
+    another."""
+    need = _select_bytes(groups, beams, vocab, beams if n_out is None else n_out)
+    return torch.zeros(need, dtype=torch.uint8, device=device)
 
 
 def decode_attention(q, kv, table, used, *, page_tokens=16, softmax_scale=None, out=None,
@@ -256,7 +283,7 @@ def decode_attention(q, kv, table, used, *, page_tokens=16, softmax_scale=None, 
     lse = q.new_empty((rows, n_q), dtype=torch.float32) if with_lse else None
     table_width = table.shape[1]
     if workspace is None:
-        workspace = _stream_workspace(device)
+        workspace = _stream_workspace("attention", device, _decode_bytes(device))
     _launch("qb_decode_attention", device, q.data_ptr(), q_ld, rows, n_q, n_kv, d, k.data_ptr(),
             v.data_ptr(), None if ks is None else ks.data_ptr(),
             None if vs is None else vs.data_ptr(), pool_rows // page_tokens, page_tokens,
@@ -271,7 +298,7 @@ def decode_attention(q, kv, table, used, *, page_tokens=16, softmax_scale=None, 
     return (result, lse) if with_lse else result
 
 
-def beam_select(logits, scores, *, finished=None, pad=0, n_out=None):
+def beam_select(logits, scores, *, finished=None, pad=0, n_out=None, workspace=None):
     """Beam search's choice over beams and vocabulary.
 
     logits: f32 or bf16 [groups * beams, vocab] (rows at any stride); scores:
@@ -279,7 +306,8 @@ def beam_select(logits, scores, *, finished=None, pad=0, n_out=None):
     beam continues only as itself, by the token pad). n_out: continuations per
     group, the beams' number when None. Returns (scores f32, parents int32,
     tokens int64), each [groups, n_out], best first; a parent is a beam's place
-    in its group.
+    in its group. workspace: from beam_workspace, for calls that never overlap;
+    the current stream's own when None.
     """
     who = "beam_select"
     if scores.dim() != 2 or scores.dtype != torch.float32 or not scores.is_contiguous():
@@ -294,18 +322,18 @@ def beam_select(logits, scores, *, finished=None, pad=0, n_out=None):
             finished.shape == scores.shape and finished.is_contiguous()
             and finished.dtype in (torch.bool, torch.uint8)):
         raise ValueError(f"{who}: finished must be contiguous bool or uint8 [groups, beams]")
-    device = _device(who, logits, scores, finished)
+    device = _device(who, logits, scores, finished, workspace)
     vocab = logits.shape[1]
-    need = ctypes.c_int64(0)
-    nat.call("qb_beam_select_workspace", groups, beams, vocab, n_out, ctypes.byref(need))
-    workspace = logits.new_empty(max(need.value, 16), dtype=torch.uint8)
+    if workspace is None:
+        workspace = _stream_workspace("select", device,
+                                      _select_bytes(groups, beams, vocab, n_out))
     score = scores.new_empty((groups, n_out))
     parent = scores.new_empty((groups, n_out), dtype=torch.int32)
     token = scores.new_empty((groups, n_out), dtype=torch.int64)
     _launch("qb_beam_select", device, logits.data_ptr(), dtype == torch.bfloat16,
             logits.stride(0) if groups * beams > 1 else vocab, groups, beams, vocab,
             scores.data_ptr(), None if finished is None else finished.data_ptr(), pad, n_out,
-            workspace.data_ptr(), need.value, score.data_ptr(), parent.data_ptr(),
+            workspace.data_ptr(), workspace.shape[0], score.data_ptr(), parent.data_ptr(),
             token.data_ptr())
     return score, parent, token
 
