@@ -10,11 +10,13 @@
 // beam first, then the beam's own order). HBM-bound: the logits are read once,
 // each block a run of one beam's; a logit costs a maximum, an exponential and
 // an addition in fp32. A block keeps its n_out best so far as sorted keys
-// (value, lower token first) and looks at single logits only where a thread's
-// largest of the current tile passes the least of them; the threads that have
-// one put it forward together, and again, until none passes. The block that
-// completes its group (a counter) joins the runs and the beams, in an order
-// that does not depend on who came last.
+// (value, lower token first). Logits that pass the least of them are put on a
+// list, without a barrier, and the list is ranked after 1, 2, 6, 22, ... tiles:
+// of a run in no order about 3 n_out pass between. Where more pass than the list
+// holds (logits that rise along the run, or many equal ones), the run is gone
+// through again tile by tile, each thread that has a logit which passes
+// putting its best forward, and again, until none does. The block that completes its group (a counter) joins the runs and the beams, in an
+// order that does not depend on who came last.
 #include "common.cuh"
 
 namespace {
@@ -27,6 +29,7 @@ constexpr int MAX_ROWS = 65535;        // groups * beams
 constexpr int THREADS = 256;
 constexpr int PER_THREAD = 16;         // logits of a thread in a tile
 constexpr int TILE = THREADS * PER_THREAD;
+constexpr int LIST = 2 * THREADS - MAX_OUT;   // keys; with the best, two a thread
 constexpr int JOIN_BYTES = 40 * 1024;  // a group's keys in the join
 constexpr float LOG2E = 1.44269504088896341f;
 
@@ -102,7 +105,7 @@ template <typename T>
 __global__ void __launch_bounds__(THREADS)
 beam_select_kernel(const SelectParams p) {
     constexpr int VE = PER_VECTOR<T>, VECTORS = PER_THREAD / VE;
-    __shared__ uint64_t s_key[MAX_OUT + THREADS];   // the best so far, in order; then new ones
+    __shared__ uint64_t s_key[MAX_OUT + LIST];   // the best so far, in order; the list
     __shared__ uint32_t s_new, s_group[32];
     __shared__ float s_m[THREADS / 32], s_s[THREADS / 32];
     __shared__ bool s_last;
@@ -124,39 +127,82 @@ beam_select_kernel(const SelectParams p) {
         if (split == p.splits - 1 && tid >= 32 && tid - 32 < tail)
             single = (int)(p.vocab - tail) + tid - 32;
         const uint4* body = reinterpret_cast<const uint4*>(x_row + head);
+        const int v0 = (int)(vectors * split / p.splits) + tid;
         const int v1 = (int)(vectors * (split + 1) / p.splits);
-        int v = (int)(vectors * split / p.splits) + tid;
+        // the run as tokens
+        const int lo = split == 0 ? 0 : head + (v0 - tid) * VE;
+        const int hi = split == p.splits - 1 ? (int)p.vocab : head + v1 * VE;
+        const float x_single = single >= 0 ? logit(x_row, single) : -INFINITY;
+
+        uint64_t least = 0;   // the last of the n_out best
+        // a logit's key where it passes, else 0. Of the logits of -inf (NaN is
+        // taken as one) only the run's first n_out places can count: any other has
+        // that many before it, equal or better.
+        auto passing = [&](float x, int index) -> uint64_t {
+            if (!(x > -INFINITY) && index - lo >= n_out) return 0;
+            const uint64_t k = offer_key(x, index);
+            return k > least ? k : 0;
+        };
+        auto put_on_list = [&](uint64_t key) {
+            if (key == 0) return;
+            const uint32_t slot = atomicAdd(&s_new, 1u);
+            if (slot < LIST) s_key[n_out + slot] = key;
+        };
+        // the n_out best of those so far and `fresh` on the list, into their
+        // places: a key's place is the number of keys above it, so the order of
+        // arrival does not matter (between barriers)
+        auto rank = [&](int fresh) {
+            const int n = n_out + fresh;
+            uint64_t mine[2];
+            int place[2];
+#pragma unroll
+            for (int c = 0; c < 2; ++c) {
+                place[c] = n_out;
+                if (tid + c * THREADS >= n) continue;
+                mine[c] = s_key[tid + c * THREADS];
+                int above = 0;
+#pragma unroll 4
+                for (int j = 0; j < n; ++j) above += s_key[j] > mine[c];
+                place[c] = above;
+            }
+            __syncthreads();
+#pragma unroll
+            for (int c = 0; c < 2; ++c)
+                if (place[c] < n_out) s_key[place[c]] = mine[c];
+            if (tid == 0) s_new = 0;
+            __syncthreads();
+            least = s_key[n_out - 1];
+        };
+        auto load = [&](uint4 (&raw)[VECTORS], int v) {
+#pragma unroll
+            for (int i = 0; i < VECTORS; ++i) {
+                raw[i] = make_uint4(0, 0, 0, 0);
+                if (v + i * THREADS < v1) raw[i] = __ldcs(body + v + i * THREADS);
+            }
+        };
 
         if (tid < n_out) s_key[tid] = n_out - tid;   // under every offer
         if (tid == 0) s_new = 0;
-        uint64_t least = 0;
         float m = -INFINITY, sum = 0.0f;
-        const float x_single = single >= 0 ? logit(x_row, single) : -INFINITY;
+        bool over = false;   // the list did not hold what passed
         uint4 raw[VECTORS];
-#pragma unroll
-        for (int i = 0; i < VECTORS; ++i) {
-            raw[i] = make_uint4(0, 0, 0, 0);
-            if (v + i * THREADS < v1) raw[i] = __ldcs(body + v + i * THREADS);
-        }
-        for (bool first = true;; first = false) {
+        load(raw, v0);
+        int at = v0;
+        for (int tile = 0, ranks = 0;; ++tile) {
+            // this thread's logits of the tile: vectors at, at + THREADS, ...
             float x[VECTORS][VE];
 #pragma unroll
             for (int i = 0; i < VECTORS; ++i) {
                 unpack(raw[i], x[i]);
-                if (v + i * THREADS >= v1)
+                if (at + i * THREADS >= v1)
 #pragma unroll
                     for (int e = 0; e < VE; ++e) x[i][e] = -INFINITY;
             }
-            const int at = v;
-            v += VECTORS * THREADS;
-            const bool more = v - tid < v1;   // (the same for the block)
-#pragma unroll
-            for (int i = 0; i < VECTORS; ++i)
-                if (v + i * THREADS < v1) raw[i] = __ldcs(body + v + i * THREADS);
-
+            const int next = at + VECTORS * THREADS;
+            load(raw, next);
             // the sum, against the largest so far
-            float top = first ? x_single : -INFINITY;
-            if (top != top) top = -INFINITY;
+            float top = -INFINITY;
+            if (tile == 0) top = fmaxf(top, x_single);
 #pragma unroll
             for (int i = 0; i < VECTORS; ++i)
 #pragma unroll
@@ -166,7 +212,7 @@ beam_select_kernel(const SelectParams p) {
                 m = top;
             }
             const float ref = m > -INFINITY ? m : 0.0f;
-            if (first && single >= 0) sum += exp_approx(x_single - ref);
+            if (tile == 0 && single >= 0) sum += exp_approx(x_single - ref);
             float part = 0.0f;
 #pragma unroll
             for (int i = 0; i < VECTORS; ++i)
@@ -174,24 +220,7 @@ beam_select_kernel(const SelectParams p) {
                 for (int e = 0; e < VE; ++e) part += exp_approx(x[i][e] - ref);
             sum += part;
 
-            // the thread's best key under `limit`
-            auto best_under = [&](uint64_t limit) {
-                uint64_t best = 0;
-#pragma unroll
-                for (int i = 0; i < VECTORS; ++i)
-#pragma unroll
-                    for (int e = 0; e < VE; ++e) {
-                        const uint64_t k =
-                            offer_key(x[i][e], head + (uint32_t)(at + i * THREADS) * VE + e);
-                        if (at + i * THREADS < v1 && k < limit && k > best) best = k;
-                    }
-                if (first && single >= 0) {
-                    const uint64_t k = offer_key(x_single, single);
-                    if (k < limit && k > best) best = k;
-                }
-                return best;
-            };
-            if (first) {
+            if (tile == 0) {
                 // n_out groups of threads or more: that many logits reach the
                 // least of their maxima, so nothing under it can be chosen
                 const bool some = at < v1 || single >= 0;
@@ -208,40 +237,58 @@ beam_select_kernel(const SelectParams p) {
                 const uint32_t g =
                     __reduce_min_sync(0xffffffffu, lane < groups ? s_group[lane] : ~0u);
                 least = g ? ((uint64_t)g << 32) - 1 : 0;   // (0: a group has no logit)
+                if (single >= 0) put_on_list(passing(x_single, single));
             }
-            uint64_t key = order_key(top) >= (uint32_t)(least >> 32) ? best_under(~0ull) : 0;
-            for (;;) {
-                const bool put = key > least;
-                const int fresh = __syncthreads_count(put);
-                if (fresh == 0) break;
-                if (put) {
-                    s_key[n_out + atomicAdd(&s_new, 1u)] = key;
-                    key = best_under(key);
-                }
-                __syncthreads();
-                // the places of the n_out best; a key's place is the number
-                // above it, so the order of arrival does not matter
-                const int n = n_out + fresh;
-                uint64_t mine[2];
-                int place[2];
+            // (a run of -inf only: its first places are in the first tile)
+            if (!over && (tile == 0 || order_key(top) >= (uint32_t)(least >> 32))) {
+                const float bar = least >> 32 ? key_value(least) : -INFINITY;
 #pragma unroll
-                for (int c = 0; c < 2; ++c) {
-                    place[c] = n_out;
-                    if (tid + c * THREADS >= n) continue;
-                    mine[c] = s_key[tid + c * THREADS];
-                    int above = 0;
-                    for (int j = 0; j < n; ++j) above += s_key[j] > mine[c];
-                    place[c] = above;
-                }
-                __syncthreads();
+                for (int i = 0; i < VECTORS; ++i)
 #pragma unroll
-                for (int c = 0; c < 2; ++c)
-                    if (place[c] < n_out) s_key[place[c]] = mine[c];
-                if (tid == 0) s_new = 0;
-                __syncthreads();
-                least = s_key[n_out - 1];
+                    for (int e = 0; e < VE; ++e)
+                        if (!(x[i][e] < bar) && at + i * THREADS < v1)
+                            put_on_list(
+                                passing(x[i][e], head + (at + i * THREADS) * VE + e));
             }
-            if (!more) break;
+            if (tile == ranks && !over) {
+                ranks = 4 * ranks + 1;
+                __syncthreads();
+                const int fresh = s_new;
+                over = fresh > LIST;
+                if (!over && fresh) rank(fresh);
+                __syncthreads();
+            }
+            at = next;
+            if (at - tid >= v1) break;   // (the same for the block)
+        }
+        __syncthreads();
+        const int fresh = s_new;
+        if (fresh > LIST) {
+            // the sure way: a tile at a time, each thread puts its best forward,
+            // in rounds
+            __syncthreads();
+            if (tid < n_out) s_key[tid] = n_out - tid;
+            if (tid == 0) s_new = 0;
+            __syncthreads();
+            least = 0;
+            for (int64_t t0 = lo; t0 < hi; t0 += TILE) {
+                const int t1 = (int)min(t0 + TILE, (int64_t)hi);
+                for (uint64_t limit = ~0ull;;) {
+                    uint64_t key = 0;
+                    for (int i = (int)t0 + tid; i < t1; i += THREADS) {
+                        const uint64_t k = passing(logit(x_row, i), i);
+                        if (k < limit && k > key) key = k;
+                    }
+                    const int put = __syncthreads_count(key != 0);
+                    if (put == 0) break;
+                    put_on_list(key);
+                    if (key) limit = key;
+                    __syncthreads();
+                    rank(put);
+                }
+            }
+        } else if (fresh) {
+            rank(fresh);
         }
         // ---- the run's results
         const float top = redux_max(m);
@@ -250,16 +297,15 @@ beam_select_kernel(const SelectParams p) {
             s_m[warp] = top;
             s_s[warp] = s;
         }
-        const int64_t at = row * p.splits + split;
-        if (tid < n_out) __stcg(p.keys + at * n_out + tid, s_key[tid]);
+        const int64_t place = row * p.splits + split;
+        if (tid < n_out) __stcg(p.keys + place * n_out + tid, s_key[tid]);
         __syncthreads();
-        if (tid == 0) {
-            float all = s_m[0];
-            for (int w = 1; w < THREADS / 32; ++w) all = fmaxf(all, s_m[w]);
-            float t = 0.0f;
-            for (int w = 0; w < THREADS / 32; ++w)
-                t += s_m[w] > -INFINITY ? s_s[w] * exp_approx(s_m[w] - all) : s_s[w];
-            __stcg(p.sums + at, make_float2(all, t));
+        if (warp == 0) {
+            const float mine = lane < THREADS / 32 ? s_m[lane] : -INFINITY;
+            const float part = lane < THREADS / 32 ? s_s[lane] : 0.0f;
+            const float all = redux_max(mine);
+            const float t = warp_sum(mine > -INFINITY ? part * exp_approx(mine - all) : part);
+            if (lane == 0) __stcg(p.sums + place, make_float2(all, t));
         }
     }
     // ---- the group's last block joins
@@ -274,22 +320,22 @@ beam_select_kernel(const SelectParams p) {
     __syncthreads();
     if (!s_last) return;
     const int64_t row0 = group * p.beams;
-    const int list = p.splits * n_out;
+    const int list = p.splits * n_out, runs = p.beams * p.splits;
+    float2* s_sums = reinterpret_cast<float2*>(s_lists + p.beams * list);
     for (int i = tid; i < p.beams * list; i += THREADS)
         s_lists[i] = __ldcg(p.keys + row0 * list + i);
+    for (int i = tid; i < runs; i += THREADS) s_sums[i] = __ldcg(p.sums + row0 * p.splits + i);
     __syncthreads();
     for (int b = warp; b < p.beams; b += THREADS / 32) {
         if (p.finished && p.finished[row0 + b]) continue;
         // lse, then the beam's offers in order, over its first run's keys
+        const float2* sums = s_sums + b * p.splits;
         float m = -INFINITY;
-        for (int i = lane; i < p.splits; i += 32)
-            m = fmaxf(m, __ldcg(p.sums + (row0 + b) * p.splits + i).x);
+        for (int i = lane; i < p.splits; i += 32) m = fmaxf(m, sums[i].x);
         m = redux_max(m);
         float sum = 0.0f;
-        for (int i = lane; i < p.splits; i += 32) {
-            const float2 part = __ldcg(p.sums + (row0 + b) * p.splits + i);
-            sum += part.x > -INFINITY ? part.y * exp_approx(part.x - m) : part.y;
-        }
+        for (int i = lane; i < p.splits; i += 32)
+            sum += sums[i].x > -INFINITY ? sums[i].y * exp_approx(sums[i].x - m) : sums[i].y;
         sum = warp_sum(sum);
         if (lane == 0) s_lse[b] = m + logf(sum);
         if (p.splits > 1) {
@@ -341,7 +387,7 @@ int select_splits(int64_t rows, int beams, int64_t vocab, int n_out) {
     const int64_t tiles = (vocab + TILE - 1) / TILE;
     int64_t splits = 740 / rows;
     splits = splits < tiles ? splits : tiles;
-    const int64_t most = JOIN_BYTES / 8 / ((int64_t)beams * n_out);
+    const int64_t most = JOIN_BYTES / 8 / ((int64_t)beams * (n_out + 1));
     splits = splits < most ? splits : most;
     return splits < 1 ? 1 : (int)splits;
 }
@@ -492,7 +538,7 @@ extern "C" int qb_beam_select(const void* logits, int logits_bf16, int64_t logit
     p.parent_out = parent_out;
     p.token_out = token_out;
     const dim3 grid((unsigned)p.splits, (unsigned)rows);
-    const int bytes = beams * p.splits * n_out * 8;
+    const int bytes = beams * p.splits * (n_out + 1) * 8;
     if (logits_bf16)
         beam_select_kernel<bf16><<<grid, THREADS, bytes, (cudaStream_t)stream>>>(p);
     else
