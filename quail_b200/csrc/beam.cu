@@ -10,9 +10,10 @@
 // beam first, then the beam's own order). HBM-bound: the logits are read once,
 // each block a run of one beam's; a logit costs a maximum, an exponential and
 // an addition in fp32. A block keeps its n_out best so far as sorted keys
-// (value, lower token first). Logits that pass the least of them are put on a
-// list, without a barrier, and the list is ranked after 1, 2, 6, 22, ... tiles:
-// of a run in no order about 3 n_out pass between. Where more pass than the list
+// (value, lower token first), and a bar: first the n_out-th largest of the
+// first tile's maxima of 8 threads, later the last of the best. Logits that
+// pass are put on a list, without a barrier, and the list is ranked after 9,
+// 81, ... tiles and at the end: of a run in no order about 8 n_out pass between. Where more pass than the list
 // holds (logits that rise along the run, or many equal ones), the run is gone
 // through again tile by tile, each thread that has a logit which passes
 // putting its best forward, and again, until none does. The block that completes its group (a counter) joins the runs and the beams, in an
@@ -27,8 +28,7 @@ constexpr int MAX_BEAMS = 32;
 constexpr int MAX_OUT = 32;
 constexpr int MAX_ROWS = 65535;        // groups * beams
 constexpr int THREADS = 256;
-constexpr int PER_THREAD = 16;         // logits of a thread in a tile
-constexpr int TILE = THREADS * PER_THREAD;
+constexpr int VECTORS = 4;             // 16-byte vectors of a thread in a tile
 constexpr int LIST = 2 * THREADS - MAX_OUT;   // keys; with the best, two a thread
 constexpr int JOIN_BYTES = 40 * 1024;  // a group's keys in the join
 constexpr float LOG2E = 1.44269504088896341f;
@@ -70,16 +70,49 @@ __device__ __forceinline__ float exp_approx(float x) {
     return r;
 }
 
-// A 16-byte vector of logits as floats
+// A 16-byte vector of logits: how many, all -inf, the largest (NaN passed
+// over), the sum of e^(x - ref), and as floats.
 template <typename T>
-constexpr int PER_VECTOR = 16 / sizeof(T);
-__device__ __forceinline__ void unpack(const uint4& v, float (&x)[4]) {
-    x[0] = __uint_as_float(v.x);
-    x[1] = __uint_as_float(v.y);
-    x[2] = __uint_as_float(v.z);
-    x[3] = __uint_as_float(v.w);
+struct Vector;
+template <>
+struct Vector<float> {
+    static constexpr int N = 4;
+    static constexpr uint32_t NONE = 0xFF800000u;
+    static __device__ __forceinline__ float at(const uint4& v, int i) {
+        return __uint_as_float(i == 0 ? v.x : i == 1 ? v.y : i == 2 ? v.z : v.w);
+    }
+    static __device__ __forceinline__ float top(const uint4& v) {
+        return fmax3(at(v, 0), at(v, 1), fmaxf(at(v, 2), at(v, 3)));
+    }
+};
+template <>
+struct Vector<bf16> {
+    static constexpr int N = 8;
+    static constexpr uint32_t NONE = 0xFF80FF80u;
+    static __device__ __forceinline__ float at(const uint4& v, int i) {
+        const uint32_t w = i < 2 ? v.x : i < 4 ? v.y : i < 6 ? v.z : v.w;
+        return __uint_as_float(i & 1 ? w & 0xFFFF0000u : w << 16);
+    }
+    static __device__ __forceinline__ float top(const uint4& v) {
+        const bf162* h = reinterpret_cast<const bf162*>(&v);
+        const bf162 m = __hmax2(__hmax2(h[0], h[1]), __hmax2(h[2], h[3]));
+        return fmaxf(__low2float(m), __high2float(m));
+    }
+};
+// + e^(x - ref) of two logits each, as pairs
+template <typename T>
+__device__ __forceinline__ void add_exps(const uint4& v, uint64_t ref, uint64_t& sum) {
+    const uint64_t scale = f2pack(LOG2E, LOG2E);
+#pragma unroll
+    for (int i = 0; i < Vector<T>::N; i += 2) {
+        float a, b;
+        f2unpack(f2mul(f2sub(f2pack(Vector<T>::at(v, i), Vector<T>::at(v, i + 1)), ref), scale),
+                 a, b);
+        asm("ex2.approx.ftz.f32 %0, %0;" : "+f"(a));
+        asm("ex2.approx.ftz.f32 %0, %0;" : "+f"(b));
+        sum = f2add(sum, f2pack(a, b));
+    }
 }
-__device__ __forceinline__ void unpack(const uint4& v, float (&x)[8]) { bf16x8_to_float(v, x); }
 __device__ __forceinline__ float logit(const float* row, int64_t i) { return row[i]; }
 __device__ __forceinline__ float logit(const bf16* row, int64_t i) {
     return __bfloat162float(row[i]);
@@ -102,11 +135,12 @@ struct SelectParams {
 
 // Block (split, row): a run of one beam's logits.
 template <typename T>
-__global__ void __launch_bounds__(THREADS)
+__global__ void __launch_bounds__(THREADS, 4)
 beam_select_kernel(const SelectParams p) {
-    constexpr int VE = PER_VECTOR<T>, VECTORS = PER_THREAD / VE;
+    constexpr int VE = Vector<T>::N, TILE = VECTORS * VE * THREADS;
     __shared__ uint64_t s_key[MAX_OUT + LIST];   // the best so far, in order; the list
-    __shared__ uint32_t s_new, s_group[32];
+    __shared__ __align__(16) uint32_t s_group[THREADS / 8];
+    __shared__ uint32_t s_new;
     __shared__ float s_m[THREADS / 32], s_s[THREADS / 32];
     __shared__ bool s_last;
     __shared__ float s_lse[MAX_BEAMS];
@@ -154,18 +188,20 @@ beam_select_kernel(const SelectParams p) {
         auto rank = [&](int fresh) {
             const int n = n_out + fresh;
             uint64_t mine[2];
-            int place[2];
+            int place[2] = {n_out, n_out};
 #pragma unroll
             for (int c = 0; c < 2; ++c) {
-                place[c] = n_out;
                 if (tid + c * THREADS >= n) continue;
                 mine[c] = s_key[tid + c * THREADS];
                 int above = 0;
-#pragma unroll 4
+#pragma unroll 8
                 for (int j = 0; j < n; ++j) above += s_key[j] > mine[c];
                 place[c] = above;
             }
-            __syncthreads();
+            if (n > 32)
+                __syncthreads();
+            else
+                __syncwarp();   // one warp holds them all
 #pragma unroll
             for (int c = 0; c < 2; ++c)
                 if (place[c] < n_out) s_key[place[c]] = mine[c];
@@ -176,87 +212,93 @@ beam_select_kernel(const SelectParams p) {
         auto load = [&](uint4 (&raw)[VECTORS], int v) {
 #pragma unroll
             for (int i = 0; i < VECTORS; ++i) {
-                raw[i] = make_uint4(0, 0, 0, 0);
+                constexpr uint32_t none = Vector<T>::NONE;
+                raw[i] = make_uint4(none, none, none, none);
                 if (v + i * THREADS < v1) raw[i] = __ldcs(body + v + i * THREADS);
             }
         };
 
         if (tid < n_out) s_key[tid] = n_out - tid;   // under every offer
         if (tid == 0) s_new = 0;
-        float m = -INFINITY, sum = 0.0f;
-        bool over = false;   // the list did not hold what passed
-        uint4 raw[VECTORS];
-        load(raw, v0);
+        float m = -INFINITY;
+        uint64_t sums = 0;    // two
+        bool over = false;    // the list did not hold what passed
+        uint4 raw[VECTORS], ahead[VECTORS];
+        load(ahead, v0);
         int at = v0;
-        for (int tile = 0, ranks = 0;; ++tile) {
+        for (int tile = 0, ranks = 8;; ++tile) {
             // this thread's logits of the tile: vectors at, at + THREADS, ...
-            float x[VECTORS][VE];
+#pragma unroll
+            for (int i = 0; i < VECTORS; ++i) raw[i] = ahead[i];
+            const int next = at + VECTORS * THREADS;
+            load(ahead, next);
+            // the sum, against the largest so far
+            float tops[VECTORS], top = tile == 0 ? fmaxf(x_single, -INFINITY) : -INFINITY;
 #pragma unroll
             for (int i = 0; i < VECTORS; ++i) {
-                unpack(raw[i], x[i]);
-                if (at + i * THREADS >= v1)
-#pragma unroll
-                    for (int e = 0; e < VE; ++e) x[i][e] = -INFINITY;
+                tops[i] = Vector<T>::top(raw[i]);
+                top = fmaxf(top, tops[i]);
             }
-            const int next = at + VECTORS * THREADS;
-            load(raw, next);
-            // the sum, against the largest so far
-            float top = -INFINITY;
-            if (tile == 0) top = fmaxf(top, x_single);
-#pragma unroll
-            for (int i = 0; i < VECTORS; ++i)
-#pragma unroll
-                for (int e = 0; e < VE; ++e) top = fmaxf(top, x[i][e]);
             if (top > m) {
-                sum *= exp_approx(m - top);
+                const float down = exp_approx(m - top);
+                sums = f2mul(sums, f2pack(down, down));
                 m = top;
             }
             const float ref = m > -INFINITY ? m : 0.0f;
-            if (tile == 0 && single >= 0) sum += exp_approx(x_single - ref);
-            float part = 0.0f;
+            if (tile == 0 && single >= 0)
+                sums = f2add(sums, f2pack(exp_approx(x_single - ref), 0.0f));
 #pragma unroll
-            for (int i = 0; i < VECTORS; ++i)
-#pragma unroll
-                for (int e = 0; e < VE; ++e) part += exp_approx(x[i][e] - ref);
-            sum += part;
+            for (int i = 0; i < VECTORS; ++i) add_exps<T>(raw[i], f2pack(ref, ref), sums);
 
             if (tile == 0) {
-                // n_out groups of threads or more: that many logits reach the
-                // least of their maxima, so nothing under it can be chosen
+                // the n_out-th largest of 32 groups' maxima: that many logits
+                // reach it, so nothing under it can be chosen
                 const bool some = at < v1 || single >= 0;
-                const uint32_t mine = some ? order_key(top) : 0u;
-                if (n_out <= THREADS / 32) {
-                    const uint32_t g = __reduce_max_sync(0xffffffffu, mine);
-                    if (lane == 0) s_group[warp] = g;
-                } else {
-                    const uint32_t g = __reduce_max_sync(0xFFu << (lane & 24), mine);
-                    if (lane % 8 == 0) s_group[tid / 8] = g;
-                }
+                uint32_t mine = some ? order_key(top) : 0u;
+#pragma unroll
+                for (int o = 1; o < 8; o <<= 1)
+                    mine = max(mine, __shfl_xor_sync(0xffffffffu, mine, o));
+                if (lane % 8 == 0) s_group[tid / 8] = mine;
                 __syncthreads();
-                const int groups = n_out <= THREADS / 32 ? THREADS / 32 : 32;
+                mine = s_group[lane];
+                int above = 0;
+                const uint4* all = reinterpret_cast<const uint4*>(s_group);
+#pragma unroll 2
+                for (int j = 0; j < 8; ++j) {
+                    const uint4 g = all[j];
+                    above += (g.x > mine) + (g.y > mine) + (g.z > mine) + (g.w > mine);
+                }
                 const uint32_t g =
-                    __reduce_min_sync(0xffffffffu, lane < groups ? s_group[lane] : ~0u);
+                    __reduce_min_sync(0xffffffffu, above < n_out ? mine : ~0u);
                 least = g ? ((uint64_t)g << 32) - 1 : 0;   // (0: a group has no logit)
                 if (single >= 0) put_on_list(passing(x_single, single));
             }
             // (a run of -inf only: its first places are in the first tile)
             if (!over && (tile == 0 || order_key(top) >= (uint32_t)(least >> 32))) {
                 const float bar = least >> 32 ? key_value(least) : -INFINITY;
+                uint32_t found = 0;   // the thread's logits that do; seldom more than one
 #pragma unroll
                 for (int i = 0; i < VECTORS; ++i)
+                    if (at + i * THREADS < v1 && !(tops[i] < bar))
 #pragma unroll
-                    for (int e = 0; e < VE; ++e)
-                        if (!(x[i][e] < bar) && at + i * THREADS < v1)
-                            put_on_list(
-                                passing(x[i][e], head + (at + i * THREADS) * VE + e));
+                        for (int e = 0; e < VE; ++e)
+                            found |= Vector<T>::at(raw[i], e) < bar ? 0u : 1u << (i * VE + e);
+                for (; found; found &= found - 1) {
+                    const int j = __ffs(found) - 1, i = j / VE;
+                    const uint4 v = i == 0 ? raw[0] : i == 1 ? raw[1] : i == 2 ? raw[2] : raw[3];
+                    put_on_list(passing(Vector<T>::at(v, j % VE),
+                                        head + (at + i * THREADS) * VE + j % VE));
+                }
             }
             if (tile == ranks && !over) {
-                ranks = 4 * ranks + 1;
+                ranks = 9 * ranks + 8;
                 __syncthreads();
                 const int fresh = s_new;
                 over = fresh > LIST;
-                if (!over && fresh) rank(fresh);
-                __syncthreads();
+                if (!over && fresh)
+                    rank(fresh);
+                else
+                    __syncthreads();   // s_new has been read
             }
             at = next;
             if (at - tid >= v1) break;   // (the same for the block)
@@ -291,6 +333,9 @@ beam_select_kernel(const SelectParams p) {
             rank(fresh);
         }
         // ---- the run's results
+        float sum, second;
+        f2unpack(sums, sum, second);
+        sum += second;
         const float top = redux_max(m);
         const float s = warp_sum(m > -INFINITY ? sum * exp_approx(m - top) : sum);
         if (lane == 0) {
@@ -381,11 +426,11 @@ beam_select_kernel(const SelectParams p) {
     }
 }
 
-// Runs that a beam's logits are cut into: about five blocks an SM, no run
-// under a tile, and the group's keys in the join's shared memory.
+// Runs that a beam's logits are cut into: one wave of four blocks an SM, no run
+// under 16 logits a thread, and the group's keys in the join's shared memory.
 int select_splits(int64_t rows, int beams, int64_t vocab, int n_out) {
-    const int64_t tiles = (vocab + TILE - 1) / TILE;
-    int64_t splits = 740 / rows;
+    const int64_t tiles = (vocab + 16 * THREADS - 1) / (16 * THREADS);
+    int64_t splits = 592 / rows;
     splits = splits < tiles ? splits : tiles;
     const int64_t most = JOIN_BYTES / 8 / ((int64_t)beams * (n_out + 1));
     splits = splits < most ? splits : most;
