@@ -440,27 +440,31 @@ int select_splits(int64_t rows, int beams, int64_t vocab, int n_out) {
 // ---- reordering -------------------------------------------------------------
 
 constexpr int COPY_THREADS = 256;
+constexpr int COPY_BATCH = 4;   // slabs whose pieces are in flight together
 
-// Whose private pages the child `j` takes: its parent's own when it is the
-// parent's first child, else those of a beam without children (the e-th such
-// child the e-th such beam). All lanes of a warp; parent is lane's own.
+// Whose private pages the child of each lane takes: its parent's own when it
+// is the parent's first child, else those of a beam without children (the
+// e-th such child the e-th such beam). All lanes of a warp; parent is the
+// lane's own.
 __device__ __forceinline__ void plan_child(int parent, int beams, int lane, int& donor,
                                            bool& moved) {
-    const uint32_t all = 0xffffffffu;
+    const uint32_t all = 0xffffffffu, below = (1u << lane) - 1u;
     const bool live = lane < beams;
-    uint32_t same = __match_any_sync(all, live ? parent : -1 - lane);
-    moved = live && (same & ((1u << lane) - 1u)) != 0;
-    uint32_t children = 0;   // beams that have one
-    for (int j = 0; j < beams; ++j) children |= 1u << __shfl_sync(all, parent, j);
+    const uint32_t same = __match_any_sync(all, live ? parent : -1 - lane);
+    moved = live && (same & below) != 0;
     const uint32_t movers = __ballot_sync(all, moved);
-    const uint32_t idle = ~children & (beams == 32 ? all : (1u << beams) - 1u);
-    const int e = __popc(movers & ((1u << lane) - 1u));
+    uint32_t idle = ~__reduce_or_sync(all, live ? 1u << parent : 0u);
     donor = parent;
-    if (moved) donor = __fns(idle, 0, e + 1);
+    if (moved) {
+        for (int e = __popc(movers & below); e > 0; --e) idle &= idle - 1;
+        donor = __ffs(idle) - 1;
+    }
 }
 
-// Block (slab, row): block 0 of a row writes its table; each block copies the
-// started page's tokens of one slab (a layer's K or V) for a child that moved.
+// Block (share, row): block 0 of a row writes its table; each copies its share
+// of the started page's tokens, over all slabs (a layer's K or V), for a child
+// that moved. HBM-bound: a moved child's started tokens are read and written
+// once.
 __global__ void __launch_bounds__(COPY_THREADS)
 beam_reorder_kernel(const int32_t* __restrict__ parents, const int32_t* __restrict__ used,
                     int beams, const int32_t* __restrict__ table_in, int64_t width,
@@ -468,61 +472,69 @@ beam_reorder_kernel(const int32_t* __restrict__ parents, const int32_t* __restri
                     int64_t row_bytes, char* pool2, int64_t row_bytes2,
                     int32_t* __restrict__ table_out, int64_t* __restrict__ next_row,
                     uint32_t* status) {
-    __shared__ int s_parent, s_donor, s_moved;
     const int64_t row = blockIdx.y, group = row / beams, first = group * beams;
-    const int child = (int)(row % beams), lane = threadIdx.x;
-    if (lane < 32) {
-        int parent = lane < beams ? parents[first + lane] : 0;
-        const bool bad = parent < 0 || parent >= beams;
-        if (bad) parent = lane;   // flagged, and taken as its own parent
-        if (bad && blockIdx.x == 0) atomicOr(status, STATUS_BAD_INDEX);
-        int donor;
-        bool moved;
-        plan_child(parent, beams, lane, donor, moved);
-        if (lane == child) {
-            s_parent = parent;
-            s_donor = donor;
-            s_moved = moved;
-        }
-    }
-    __syncthreads();
-    const int32_t* from = table_in + (first + s_parent) * width;
-    const int32_t* own = table_in + (first + s_donor) * width;
+    const int child = (int)(row - first), lane = threadIdx.x & 31;
+    const bool leader = blockIdx.x == 0 && threadIdx.x == 0;
     const int n = used[group];
+    // every warp plans for itself
+    int parent = lane < beams ? parents[first + lane] : 0, donor;
+    const bool bad = parent < 0 || parent >= beams;
+    if (bad) parent = lane;   // flagged, and taken as its own parent
+    if (bad && blockIdx.x == 0 && threadIdx.x < 32) atomicOr(status, STATUS_BAD_INDEX);
+    bool moved;
+    plan_child(parent, beams, lane, donor, moved);
+    parent = __shfl_sync(0xffffffffu, parent, child);
+    donor = __shfl_sync(0xffffffffu, donor, child);
+    moved = __shfl_sync(0xffffffffu, moved, child);
+
+    const int32_t* from = table_in + (first + parent) * width;
+    const int32_t* own = table_in + (first + donor) * width;
     const int64_t full = n < 0 ? 0 : n / page_tokens;
-    if (n < 0 || full > width || (full == width && n % page_tokens)) {
-        if (threadIdx.x == 0 && blockIdx.x == 0) {
-            atomicOr(status, STATUS_BAD_INDEX);
-            if (next_row) next_row[row] = -1;
-        }
-        if (blockIdx.x == 0)
-            for (int64_t i = threadIdx.x; i < width; i += COPY_THREADS)
-                table_out[row * width + i] = from[i];
-        return;
-    }
-    const int tail = n % page_tokens;
+    const int tail = n < 0 ? 0 : n % page_tokens;
+    const bool fits = n >= 0 && (full < width || (full == width && tail == 0));
+    if (leader && !fits) atomicOr(status, STATUS_BAD_INDEX);
     if (blockIdx.x == 0) {
         for (int64_t i = threadIdx.x; i < width; i += COPY_THREADS)
-            table_out[row * width + i] = i < full ? from[i] : own[i];
+            table_out[row * width + i] = i < full || !fits ? from[i] : own[i];
         if (next_row && threadIdx.x == 0)
-            next_row[row] = full < width ? (int64_t)own[full] * page_tokens + tail : -1;
+            next_row[row] =
+                fits && full < width ? (int64_t)own[full] * page_tokens + tail : -1;
     }
-    if (!s_moved || tail == 0) return;
+    if (!fits || !moved || tail == 0) return;
     const int64_t src = from[full], dst = own[full];
     if (src < 0 || src >= n_pages || dst < 0 || dst >= n_pages) {
-        if (threadIdx.x == 0) atomicOr(status, STATUS_BAD_INDEX);
+        if (leader) atomicOr(status, STATUS_BAD_INDEX);
         return;
     }
-    for (int64_t slab = blockIdx.x; slab < n_slabs; slab += gridDim.x) {
-        const int64_t base = slab * n_pages * page_tokens;
-        const char* a = pool + (base + src * page_tokens) * row_bytes;
-        char* b = pool + (base + dst * page_tokens) * row_bytes;
-        for (int64_t i = threadIdx.x * 16; i < tail * row_bytes; i += COPY_THREADS * 16)
-            *reinterpret_cast<uint4*>(b + i) = *reinterpret_cast<const uint4*>(a + i);
-        if (pool2) {   // scale bytes: few, and rows of any width
-            a = pool2 + (base + src * page_tokens) * row_bytes2;
-            b = pool2 + (base + dst * page_tokens) * row_bytes2;
-            for (int64_t i = threadIdx.x; i < tail * row_bytes2; i += COPY_THREADS) b[i] = a[i];
+    // the slabs share, share + shares, ...; a piece of several at a time
+    const int64_t slab_rows = n_pages * page_tokens, slab_bytes = slab_rows * row_bytes;
+    const int share = blockIdx.x, shares = gridDim.x, slabs = (int)n_slabs;
+    const int pieces = (int)(tail * row_bytes / 16);
+    const char* a = pool + src * page_tokens * row_bytes;
+    char* b = pool + dst * page_tokens * row_bytes;
+    for (int slab0 = share; slab0 < slabs; slab0 += shares * COPY_BATCH)
+        for (int i = threadIdx.x; i < pieces; i += COPY_THREADS) {
+            uint4 held[COPY_BATCH];
+#pragma unroll
+            for (int j = 0; j < COPY_BATCH; ++j)
+                if (slab0 + j * shares < slabs)
+                    held[j] = *reinterpret_cast<const uint4*>(
+                        a + (slab0 + j * shares) * slab_bytes + i * 16LL);
+#pragma unroll
+            for (int j = 0; j < COPY_BATCH; ++j)
+                if (slab0 + j * shares < slabs)
+                    *reinterpret_cast<uint4*>(b + (slab0 + j * shares) * slab_bytes +
+                                              i * 16LL) = held[j];
+        }
+    if (pool2) {   // scale bytes: few, and rows of any width
+        const int64_t bytes = tail * row_bytes2, all = n_slabs * bytes;
+        a = pool2 + src * page_tokens * row_bytes2;
+        b = pool2 + dst * page_tokens * row_bytes2;
+        for (int64_t i = (int64_t)blockIdx.x * COPY_THREADS + threadIdx.x; i < all;
+             i += (int64_t)gridDim.x * COPY_THREADS) {
+            const int64_t slab = i / bytes;
+            const int64_t byte = slab * slab_rows * row_bytes2 + i - slab * bytes;
+            b[byte] = a[byte];
         }
     }
 }
@@ -601,8 +613,8 @@ extern "C" int qb_beam_reorder(const int32_t* parents, const int32_t* used, int6
     if (groups < 0 || groups * beams > 65535)
         return invalid("qb_beam_reorder: 0 to 65,535 rows");
     if (page_tokens <= 0 || page_tokens > 1024 || n_pages <= 0 || table_width <= 0 ||
-        n_slabs < 0)
-        return invalid("qb_beam_reorder: bad page, table or slab counts");
+        n_slabs < 0 || n_slabs > (1 << 20) || row_bytes > (1 << 20))
+        return invalid("qb_beam_reorder: bad page, table, slab or row sizes");
     if (n_slabs > 0 && (!pool || row_bytes <= 0 || row_bytes % 16 || !aligned(pool, 16)))
         return invalid("qb_beam_reorder: pool rows must be multiples of 16 bytes, 16-byte aligned");
     if (pool2 && row_bytes2 <= 0) return invalid("qb_beam_reorder: row_bytes2 must be positive");
@@ -612,8 +624,13 @@ extern "C" int qb_beam_reorder(const int32_t* parents, const int32_t* used, int6
     if (table_in == table_out) return invalid("qb_beam_reorder: table_out must not be table_in");
     uint32_t* status = device_status_ptr();
     if (!status) return launch_status("qb_beam_reorder: status word");
-    const int64_t slabs = n_slabs < 1 ? 1 : n_slabs < 1024 ? n_slabs : 1024;
-    const dim3 grid((unsigned)slabs, (unsigned)(groups * beams));
+    // shares of a row's slabs: a few waves of blocks, each with a batch where the
+    // slabs suffice
+    const int64_t rows = groups * beams;
+    int64_t shares = 148 * 16 / rows;
+    shares = shares < n_slabs ? shares : n_slabs;
+    shares = shares < 1 ? 1 : shares;
+    const dim3 grid((unsigned)shares, (unsigned)rows);
     beam_reorder_kernel<<<grid, COPY_THREADS, 0, (cudaStream_t)stream>>>(
         parents, used, beams, table_in, table_width, page_tokens, n_pages, (char*)pool, n_slabs,
         row_bytes, (char*)pool2, row_bytes2, table_out, next_row, status);
