@@ -15,6 +15,7 @@ here (ValueError); sizes, strides and alignment by the library.
 """
 
 import ctypes
+import functools
 from typing import NamedTuple
 
 import torch
@@ -58,22 +59,29 @@ class QuantKV:
         return self.codes, self.scales
 
 
-def _launch(name, device, *args):
-    """One library call on the current stream of CUDA device `device`."""
-    stream = torch._C._cuda_getCurrentRawStream(device)
-    if device == torch._C._cuda_getDevice():
-        nat.call(name, *args, stream)
-    else:
+_bf16, _f32, _i32, _i64 = torch.bfloat16, torch.float32, torch.int32, torch.int64
+_current_device, _raw_stream = torch._C._cuda_getDevice, torch._C._cuda_getCurrentRawStream
+
+
+def _launch(name, device, args):
+    """One library call (the arguments before the stream) on the current stream
+    of CUDA device `device`. nat.call without its look-ups: a call's host time is
+    what a small one costs."""
+    if device != _current_device():
         with torch.cuda.device(device):
-            nat.call(name, *args, stream)
+            return _launch(name, device, args)
+    status = getattr(nat.load(), name)(*args, _raw_stream(device))
+    if status:
+        nat.check(status, name)
+    nat.LAUNCHES["count"] += 1
 
 
-def _device(who, *tensors):
+def _device(who, first, *others):
     """The index of the one CUDA device that holds the tensors (None skipped)."""
-    device = tensors[0].get_device()
+    device = first.get_device()
     if device < 0:
         raise ValueError(f"{who}: CUDA tensors are needed")
-    for t in tensors:
+    for t in others:
         if t is not None and t.get_device() != device:
             raise ValueError(f"{who}: tensors on different devices")
     return device
@@ -82,9 +90,10 @@ def _device(who, *tensors):
 def _heads(who, name, x):
     """(rows, heads, d, row stride) of bf16 rows of heads [rows, n, d], each
     row's heads contiguous."""
-    if x.dim() != 3 or x.dtype != torch.bfloat16:
+    shape = x.shape
+    if len(shape) != 3 or x.dtype != _bf16:
         raise ValueError(f"{who}: {name} must be bf16 [rows, n, d]")
-    rows, n, d = x.shape
+    rows, n, d = shape
     ld, head, one = x.stride()
     if one != 1 or (head != d and n > 1):
         raise ValueError(f"{who}: the heads of a row of {name} must be contiguous")
@@ -106,8 +115,9 @@ def _quant_layer(who, kv):
 
 
 def _index(who, name, x, n=None):
-    if x.dtype != torch.int64 or x.dim() != 1 or not x.is_contiguous() or (
-            n is not None and x.shape[0] != n):
+    shape = x.shape
+    if x.dtype != _i64 or len(shape) != 1 or not x.is_contiguous() or (
+            n is not None and shape[0] != n):
         raise ValueError(f"{who}: {name} must be a contiguous int64 vector as long as the rows")
 
 
@@ -138,10 +148,10 @@ def kv_quant_write(k, v, kv: QuantLayer, dst, src=None):
     n = rows if src is None else src.shape[0]
     _index(who, "dst", dst, n)
     device = _device(who, k, v, dst, src, *kv)
-    _launch("qb_kv_quant_write", device, k.data_ptr(), v.data_ptr(), k_ld, v_ld,
-            None if src is None else src.data_ptr(), dst.data_ptr(), n, rows, n_kv, d,
-            kv.k.data_ptr(), kv.v.data_ptr(), kv.k_scale.data_ptr(), kv.v_scale.data_ptr(),
-            pool_rows)
+    _launch("qb_kv_quant_write", device, (
+        k.data_ptr(), v.data_ptr(), k_ld, v_ld, None if src is None else src.data_ptr(),
+        dst.data_ptr(), n, rows, n_kv, d, kv.k.data_ptr(), kv.v.data_ptr(),
+        kv.k_scale.data_ptr(), kv.v_scale.data_ptr(), pool_rows))
 
 
 def kv_quant_read(kv: QuantLayer, src, dst=None, out=None):
@@ -164,10 +174,10 @@ def kv_quant_read(kv: QuantLayer, src, dst=None, out=None):
         if dst is not None:
             _index(who, "dst", dst, n)
     device = _device(who, k, v, src, dst, *kv)
-    _launch("qb_kv_quant_read", device, kv.k.data_ptr(), kv.v.data_ptr(),
-            kv.k_scale.data_ptr(), kv.v_scale.data_ptr(), pool_rows, src.data_ptr(),
-            None if dst is None else dst.data_ptr(), n, n_kv, d, k.data_ptr(), v.data_ptr(),
-            k_ld, v_ld, rows)
+    _launch("qb_kv_quant_read", device, (
+        kv.k.data_ptr(), kv.v.data_ptr(), kv.k_scale.data_ptr(), kv.v_scale.data_ptr(),
+        pool_rows, src.data_ptr(), None if dst is None else dst.data_ptr(), n, n_kv, d,
+        k.data_ptr(), v.data_ptr(), k_ld, v_ld, rows))
     return k, v
 
 
@@ -212,6 +222,7 @@ def decode_workspace(device="cuda"):
     return torch.zeros(_decode_bytes(index), dtype=torch.uint8, device=device)
 
 
+@functools.lru_cache(maxsize=256)
 def _select_bytes(groups, beams, vocab, n_out):
     need = ctypes.c_int64(0)
     nat.call("qb_beam_select_workspace", groups, beams, vocab, n_out, ctypes.byref(need))
@@ -248,19 +259,20 @@ def decode_attention(q, kv, table, used, *, page_tokens=16, softmax_scale=None, 
     else:
         k, v = kv
         ks = vs = None
-        if not (k.dim() == 3 and k.shape == v.shape and k.dtype == v.dtype == torch.bfloat16
+        shape = k.shape
+        if not (len(shape) == 3 and v.shape == shape and k.dtype == v.dtype == _bf16
                 and k.is_contiguous() and v.is_contiguous()):
             raise ValueError(f"{who}: bf16 pools must be contiguous [rows, n_kv, d]")
-        pool_rows, n_kv, width = k.shape
+        pool_rows, n_kv, width = shape
     if width != d:
         raise ValueError(f"{who}: q's head size is not the cache's")
-    if pool_rows % page_tokens:
+    if page_tokens <= 0 or pool_rows % page_tokens:
         raise ValueError(f"{who}: the pools are not whole pages")
-    if table.dim() != 2 or table.dtype != torch.int32 or table.shape[0] != rows or (
-            table.stride(1) != 1):
+    shape = table.shape
+    if len(shape) != 2 or shape[0] != rows or table.dtype != _i32 or table.stride(1) != 1:
         raise ValueError(f"{who}: table must be int32 [rows, pages]")
-    if used.dim() != 1 or used.dtype != torch.int32 or used.shape[0] != rows or (
-            not used.is_contiguous()):
+    table_width = shape[1]
+    if used.shape != (rows,) or used.dtype != _i32 or not used.is_contiguous():
         raise ValueError(f"{who}: used must be int32 [rows]")
     q8 = q8_scale = None
     q8_ld, ue8m0, out_ld = 0, False, 0
@@ -278,22 +290,20 @@ def decode_attention(q, kv, table, used, *, page_tokens=16, softmax_scale=None, 
         out_ld = _heads(who, "out", out)[3]
     device = _device(who, q, k, v, ks, vs, table, used, out, q8, q8_scale, workspace)
     if out is None and q8 is None:
-        out = q.new_empty((rows, n_q, d))
+        out = torch.empty_like(q, memory_format=torch.contiguous_format)
         out_ld = n_q * d
-    lse = q.new_empty((rows, n_q), dtype=torch.float32) if with_lse else None
-    table_width = table.shape[1]
+    lse = q.new_empty((rows, n_q), dtype=_f32) if with_lse else None
     if workspace is None:
         workspace = _stream_workspace("attention", device, _decode_bytes(device))
-    _launch("qb_decode_attention", device, q.data_ptr(), q_ld, rows, n_q, n_kv, d, k.data_ptr(),
-            v.data_ptr(), None if ks is None else ks.data_ptr(),
-            None if vs is None else vs.data_ptr(), pool_rows // page_tokens, page_tokens,
-            table.data_ptr(), table_width, table.stride(0) if rows > 1 else table_width,
-            used.data_ptr(), d ** -0.5 if softmax_scale is None else softmax_scale,
-            workspace.data_ptr(), workspace.shape[0],
-            None if out is None else out.data_ptr(), out_ld,
-            None if q8 is None else q8.data_ptr(),
-            None if q8 is None else q8_scale.data_ptr(), q8_ld, ue8m0,
-            None if lse is None else lse.data_ptr())
+    _launch("qb_decode_attention", device, (
+        q.data_ptr(), q_ld, rows, n_q, n_kv, d, k.data_ptr(), v.data_ptr(),
+        None if ks is None else ks.data_ptr(), None if vs is None else vs.data_ptr(),
+        pool_rows // page_tokens, page_tokens, table.data_ptr(), table_width,
+        table.stride(0) if rows > 1 else table_width, used.data_ptr(),
+        d ** -0.5 if softmax_scale is None else softmax_scale, workspace.data_ptr(),
+        workspace.shape[0], None if out is None else out.data_ptr(), out_ld,
+        None if q8 is None else q8.data_ptr(), None if q8 is None else q8_scale.data_ptr(),
+        q8_ld, ue8m0, None if lse is None else lse.data_ptr()))
     result = quantised if out is None else out
     return (result, lse) if with_lse else result
 
@@ -310,31 +320,32 @@ def beam_select(logits, scores, *, finished=None, pad=0, n_out=None, workspace=N
     the current stream's own when None.
     """
     who = "beam_select"
-    if scores.dim() != 2 or scores.dtype != torch.float32 or not scores.is_contiguous():
+    shape = scores.shape
+    if len(shape) != 2 or scores.dtype != _f32 or not scores.is_contiguous():
         raise ValueError(f"{who}: scores must be contiguous f32 [groups, beams]")
-    groups, beams = scores.shape
+    groups, beams = shape
     n_out = beams if n_out is None else n_out
-    dtype = logits.dtype
-    if logits.dim() != 2 or logits.shape[0] != groups * beams or logits.stride(1) != 1 or (
-            dtype != torch.float32 and dtype != torch.bfloat16):
+    dtype, shape = logits.dtype, logits.shape
+    if len(shape) != 2 or shape[0] != groups * beams or logits.stride(1) != 1 or (
+            dtype != _f32 and dtype != _bf16):
         raise ValueError(f"{who}: logits must be f32 or bf16 [groups * beams, vocab]")
     if finished is not None and not (
             finished.shape == scores.shape and finished.is_contiguous()
             and finished.dtype in (torch.bool, torch.uint8)):
         raise ValueError(f"{who}: finished must be contiguous bool or uint8 [groups, beams]")
     device = _device(who, logits, scores, finished, workspace)
-    vocab = logits.shape[1]
+    vocab = shape[1]
     if workspace is None:
         workspace = _stream_workspace("select", device,
                                       _select_bytes(groups, beams, vocab, n_out))
-    score = scores.new_empty((groups, n_out))
-    parent = scores.new_empty((groups, n_out), dtype=torch.int32)
-    token = scores.new_empty((groups, n_out), dtype=torch.int64)
-    _launch("qb_beam_select", device, logits.data_ptr(), dtype == torch.bfloat16,
-            logits.stride(0) if groups * beams > 1 else vocab, groups, beams, vocab,
-            scores.data_ptr(), None if finished is None else finished.data_ptr(), pad, n_out,
-            workspace.data_ptr(), workspace.shape[0], score.data_ptr(), parent.data_ptr(),
-            token.data_ptr())
+    score = torch.empty_like(scores) if n_out == beams else scores.new_empty((groups, n_out))
+    parent = scores.new_empty((groups, n_out), dtype=_i32)
+    token = scores.new_empty((groups, n_out), dtype=_i64)
+    _launch("qb_beam_select", device, (
+        logits.data_ptr(), dtype == _bf16, logits.stride(0) if groups * beams > 1 else vocab,
+        groups, beams, vocab, scores.data_ptr(),
+        None if finished is None else finished.data_ptr(), pad, n_out, workspace.data_ptr(),
+        workspace.shape[0], score.data_ptr(), parent.data_ptr(), token.data_ptr()))
     return score, parent, token
 
 
@@ -351,32 +362,35 @@ def beam_reorder(pools, parents, used, table, *, page_tokens=16):
     row of each beam's next token (-1 when its table is full).
     """
     who = "beam_reorder"
-    if parents.dim() != 2 or parents.dtype != torch.int32 or not parents.is_contiguous():
+    shape = parents.shape
+    if len(shape) != 2 or parents.dtype != _i32 or not parents.is_contiguous():
         raise ValueError(f"{who}: parents must be contiguous int32 [groups, beams]")
-    groups, beams = parents.shape
-    if used.dim() != 1 or used.shape[0] != groups or used.dtype != torch.int32 or (
-            not used.is_contiguous()):
+    groups, beams = shape
+    if used.shape != (groups,) or used.dtype != _i32 or not used.is_contiguous():
         raise ValueError(f"{who}: used must be int32 [groups]")
-    if table.dim() != 2 or table.dtype != torch.int32 or table.shape[0] != groups * beams or (
+    shape = table.shape
+    if len(shape) != 2 or shape[0] != groups * beams or table.dtype != _i32 or (
             not table.is_contiguous()):
         raise ValueError(f"{who}: table must be contiguous int32 [groups * beams, pages]")
+    width = shape[1]
     if len(pools) not in (1, 2):
         raise ValueError(f"{who}: one pool, or codes and scales")
     pool = pools[0]
     second = pools[1] if len(pools) == 2 else None
-    for x in pools:
-        if x.dim() < 4 or x.shape[:3] != pool.shape[:3] or not x.is_contiguous():
-            raise ValueError(f"{who}: pools must be contiguous [n_layers, 2, rows, ...]")
-    layers, two, rows = pool.shape[:3]
-    if rows % page_tokens:
+    shape = pool.shape
+    if len(shape) < 4 or not pool.is_contiguous() or second is not None and not (
+            second.dim() >= 4 and second.shape[:3] == shape[:3] and second.is_contiguous()):
+        raise ValueError(f"{who}: pools must be contiguous [n_layers, 2, rows, ...]")
+    rows = shape[2]
+    if page_tokens <= 0 or rows % page_tokens:
         raise ValueError(f"{who}: the pools are not whole pages")
     device = _device(who, pool, second, parents, used, table)
     out = torch.empty_like(table)
-    next_row = table.new_empty(groups * beams, dtype=torch.int64)
-    _launch("qb_beam_reorder", device, parents.data_ptr(), used.data_ptr(), groups, beams,
-            table.data_ptr(), table.shape[1], page_tokens, rows // page_tokens, pool.data_ptr(),
-            layers * two, pool.stride(2) * pool.element_size(),
-            None if second is None else second.data_ptr(),
-            0 if second is None else second.stride(2) * second.element_size(), out.data_ptr(),
-            next_row.data_ptr())
+    next_row = table.new_empty(groups * beams, dtype=_i64)
+    _launch("qb_beam_reorder", device, (
+        parents.data_ptr(), used.data_ptr(), groups, beams, table.data_ptr(), width, page_tokens,
+        rows // page_tokens, pool.data_ptr(), shape[0] * shape[1],
+        pool.stride(2) * pool.element_size(), None if second is None else second.data_ptr(),
+        0 if second is None else second.stride(2) * second.element_size(), out.data_ptr(),
+        next_row.data_ptr()))
     return out, next_row
