@@ -9,7 +9,8 @@ answers. Margins (yes - no logits) come back too, for parity checks.
 ``join`` is its AI join branch (backend.py:166-214: run_join over anchors
 and per-stage partner lists) and ``score`` the AI.SCORE reranker
 (quail/backends/quail/executor/score.py:46-66: run_join with the sigmoid
-readout).
+readout). ``generate`` continues rows by tokens, which the reference's
+prefill-only path does not (quail_b200.generate).
 """
 
 import time
@@ -19,6 +20,7 @@ import numpy as np
 
 from quail_b200 import loop
 from quail_b200.arena import KVArena
+from quail_b200.generate import Generator
 from quail_b200.loop import InputStaging
 from quail_b200.model import random_weights, requant_ue8m0, scales_are_ue8m0
 from quail_b200.pipeline import build_pipeline
@@ -101,6 +103,7 @@ class B200Executor:
         self.budget = cfg.max_chunk_tokens
         # pinned host / device input buffers reused by every chunk upload
         self.staging = InputStaging(torch, self.device)
+        self._generators = {}   # kv format -> Generator
 
     def reset_arena(self):
         """Free every page (the pools stay allocated)."""
@@ -203,3 +206,14 @@ class B200Executor:
         per = None if partners is None else [[p] for p in partners]
         return self._join(ans, anchors, [suffixes], None, budget, attention, share_prefixes,
                           per)
+
+    def generate(self, prompts, max_new_tokens, *, beams=1, eos=None, kv="bf16"):
+        """Continue each prompt (token ids) by up to max_new_tokens tokens: beam
+        search, greedy with one beam. kv: "bf16" decodes over the arena's pools,
+        "fp8" over an 8-bit copy of the prompts' KV. Returns a
+        generate.Completion (tokens and log-probability of each beam) per
+        prompt; the arena's pages are free again afterwards."""
+        held = self._generators.get(kv)
+        if held is None:
+            held = self._generators[kv] = Generator(self, kv)
+        return held.generate(prompts, max_new_tokens, beams=beams, eos=eos)

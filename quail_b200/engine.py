@@ -63,6 +63,10 @@ class Engine:
         scale = t.empty((width // GROUP, max(rows, 1)), dtype=t.float32, device="cuda")
         return QuantRows(q, scale, max(rows, 1))
 
+    def quant_rows(self, rows, width):
+        """Unwritten fp8 rows and scales for a quantising kernel to fill."""
+        return self._quant_buffers(rows, width)
+
     # ---- norms and quantisation ---------------------------------------------
 
     def embed_norm_quant(self, ids, embed, norm_w):
