@@ -3,7 +3,9 @@
 Each ``csrc/*.cu`` compiles to an object with nvcc for ``sm_100a`` only,
 and the objects link into ``quail_b200/libquailb200.so`` with the CUDA
 runtime linked statically, so the library carries no dependency on the
-runtime version torch bundles. Run as ``python -m quail_b200.build``.
+runtime version torch bundles. ``csrc/torch_ops.cpp``, the generation
+operators' torch calls over that library's C ABI, compiles with g++ to
+``quail_b200/_torch_ops.so``. Run as ``python -m quail_b200.build``.
 """
 
 import concurrent.futures
@@ -11,12 +13,14 @@ import os
 import shutil
 import subprocess
 import sys
+import sysconfig
 from pathlib import Path
 
 PACKAGE = Path(__file__).resolve().parent
 CSRC = PACKAGE / "csrc"
 INCLUDE = PACKAGE.parent / "include"
 LIBRARY = PACKAGE / "libquailb200.so"
+TORCH_OPS = PACKAGE / "_torch_ops.so"
 BUILD_DIR = PACKAGE.parent / "_build"
 
 ARCH_FLAGS = ["-gencode", "arch=compute_100a,code=sm_100a"]
@@ -62,8 +66,30 @@ def _compile(src: Path, verbose_ptxas: bool) -> Path:
     return obj
 
 
+def _build_torch_ops(force: bool) -> Path:
+    src = CSRC / "torch_ops.cpp"
+    if not force and not _stale(TORCH_OPS, [src, *INCLUDE.glob("*.h")]):
+        return TORCH_OPS
+    import torch
+    root = Path(torch.__file__).parent
+    tmp = TORCH_OPS.with_suffix(".so.tmp")
+    cmd = ["g++", "-O2", "-std=c++17", "-shared", "-fPIC",
+           f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}",
+           "-I", str(root / "include"),
+           "-I", str(root / "include" / "torch" / "csrc" / "api" / "include"),
+           "-I", sysconfig.get_paths()["include"],
+           "-I", str(Path(nvcc()).resolve().parent.parent / "include"), str(src), "-o", str(tmp),
+           "-L", str(root / "lib"), "-lc10", "-lc10_cuda", "-ltorch_cpu", "-ltorch_python"]
+    proc = subprocess.run(cmd, capture_output=True, text=True)
+    if proc.returncode != 0:
+        raise RuntimeError(f"g++ failed on {src.name}:\n{proc.stdout}\n{proc.stderr}")
+    os.replace(tmp, TORCH_OPS)
+    return TORCH_OPS
+
+
 def build(force: bool = False, verbose_ptxas: bool = False) -> Path:
-    """Compile every kernel source and link the shared library.
+    """Compile every kernel source, link the shared library and build the torch
+    calls over it.
 
     Returns:
         The path of libquailb200.so.
@@ -73,8 +99,10 @@ def build(force: bool = False, verbose_ptxas: bool = False) -> Path:
     if force:
         for obj in BUILD_DIR.glob("*.o"):
             obj.unlink()
-    with concurrent.futures.ThreadPoolExecutor(max_workers=min(8, len(srcs))) as pool:
+    with concurrent.futures.ThreadPoolExecutor(max_workers=min(8, len(srcs) + 1)) as pool:
+        torch_ops = pool.submit(_build_torch_ops, force)
         objs = list(pool.map(lambda s: _compile(s, verbose_ptxas), srcs))
+        torch_ops.result()
     if force or _stale(LIBRARY, objs):
         tmp = LIBRARY.with_suffix(".so.tmp")
         cmd = [nvcc(), *ARCH_FLAGS, "-shared", "-cudart", "static", "-o", str(tmp),
