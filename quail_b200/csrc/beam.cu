@@ -371,19 +371,22 @@ beam_select_kernel(const SelectParams p) {
         s_lists[i] = __ldcg(p.keys + row0 * list + i);
     for (int i = tid; i < runs; i += THREADS) s_sums[i] = __ldcg(p.sums + row0 * p.splits + i);
     __syncthreads();
-    for (int b = warp; b < p.beams; b += THREADS / 32) {
+    // a beam's offers in order, over its first run's keys, and then its lse: a
+    // warp each
+    for (int task = warp; task < 2 * p.beams; task += THREADS / 32) {
+        const int b = task < p.beams ? task : task - p.beams;
         if (p.finished && p.finished[row0 + b]) continue;
-        // lse, then the beam's offers in order, over its first run's keys
-        const float2* sums = s_sums + b * p.splits;
-        float m = -INFINITY;
-        for (int i = lane; i < p.splits; i += 32) m = fmaxf(m, sums[i].x);
-        m = redux_max(m);
-        float sum = 0.0f;
-        for (int i = lane; i < p.splits; i += 32)
-            sum += sums[i].x > -INFINITY ? sums[i].y * exp_approx(sums[i].x - m) : sums[i].y;
-        sum = warp_sum(sum);
-        if (lane == 0) s_lse[b] = m + logf(sum);
-        if (p.splits > 1) {
+        if (task >= p.beams) {
+            const float2* sums = s_sums + b * p.splits;
+            float m = -INFINITY;
+            for (int i = lane; i < p.splits; i += 32) m = fmaxf(m, sums[i].x);
+            m = redux_max(m);
+            float sum = 0.0f;
+            for (int i = lane; i < p.splits; i += 32)
+                sum += sums[i].x > -INFINITY ? sums[i].y * exp_approx(sums[i].x - m) : sums[i].y;
+            sum = warp_sum(sum);
+            if (lane == 0) s_lse[b] = m + logf(sum);
+        } else if (p.splits > 1) {
             uint64_t* keys = s_lists + b * list;
             uint64_t limit = ~0ull, chosen = 0;   // of rank `lane`
             for (int r = 0; r < n_out; ++r) {
@@ -429,7 +432,7 @@ beam_select_kernel(const SelectParams p) {
 // Runs that a beam's logits are cut into: one wave of four blocks an SM, no run
 // under 16 logits a thread, and the group's keys in the join's shared memory.
 int select_splits(int64_t rows, int beams, int64_t vocab, int n_out) {
-    const int64_t tiles = (vocab + 16 * THREADS - 1) / (16 * THREADS);
+    const int64_t tiles = vocab / (16 * THREADS);
     int64_t splits = 592 / rows;
     splits = splits < tiles ? splits : tiles;
     const int64_t most = JOIN_BYTES / 8 / ((int64_t)beams * (n_out + 1));

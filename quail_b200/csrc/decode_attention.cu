@@ -678,35 +678,39 @@ decode_attention_kernel(const Params p) {
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     const int per_row = p.n_kv * p.tiles;   // items of a row
 
-    // ---- a scan over the rows' units, `chunk` rows a thread
-    const int chunk = (p.rows + THREADS - 1) / THREADS;
-    const int r0 = min(tid * chunk, p.rows), r1 = min(r0 + chunk, p.rows);
+    // ---- a scan over the rows' units: up to 32 rows by every warp for itself, a
+    // row a lane; more by the block, `chunk` rows a thread
+    const bool few = p.rows <= 32;
+    const int chunk = few ? 1 : (p.rows + THREADS - 1) / THREADS;
+    const int r0 = min((few ? lane : tid) * chunk, p.rows), r1 = min(r0 + chunk, p.rows);
     int upto = 0, full = 0;
     for (int r = r0; r < r1; ++r) {
         const int n = units_of(p, row_keys(p, r, blockIdx.x == 0));
         upto += n;
         full += n > 0;
     }
+    const int own = upto;
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
         const int u = __shfl_up_sync(0xffffffffu, upto, o);
         if (lane >= o) upto += u;
     }
     full = __reduce_add_sync(0xffffffffu, full);
-    s_upto[tid] = upto;
-    if (lane == 31) {
-        s_scan[warp] = upto;
-        s_full[warp] = full;
-    }
     if (lane < 2) slots[2 * warp + lane].start = -1;
-    __syncthreads();
-    int units = 0, earlier[WARPS];   // of the warps before each
-    full = 0;
+    int units = __shfl_sync(0xffffffffu, upto, 31);
+    if (!few) {
+        s_upto[tid] = upto;
+        if (lane == 31) {
+            s_scan[warp] = upto;
+            s_full[warp] = full;
+        }
+        __syncthreads();
+        units = full = 0;
 #pragma unroll
-    for (int w = 0; w < WARPS; ++w) {
-        earlier[w] = units;
-        units += s_scan[w];
-        full += s_full[w];
+        for (int w = 0; w < WARPS; ++w) {
+            units += s_scan[w];
+            full += s_full[w];
+        }
     }
     const int total = units * per_row;
     // rows without keys
@@ -739,22 +743,28 @@ decode_attention_kernel(const Params p) {
         } else {
             at.at = cuts.at(blockIdx.x + c);
         }
-        int ended = 0, earlier = 0;
+        if (few) {
+            at.row = __popc(__ballot_sync(0xffffffffu, upto * per_row <= at.at));
+            at.before = __shfl_sync(0xffffffffu, upto - own, at.row);
+            n = __shfl_sync(0xffffffffu, own, at.row);
+        } else {
+            int ended = 0, earlier = 0;
 #pragma unroll
-        for (int w = 0; w < WARPS; ++w) {
-            ended += (earlier + s_upto[32 * w + lane]) * per_row <= at.at;
-            earlier += s_scan[w];
-        }
-        ended = __reduce_add_sync(0xffffffffu, ended);
-        at.row = ended * chunk;
-        at.before = ended ? s_upto[ended - 1] : 0;
+            for (int w = 0; w < WARPS; ++w) {
+                ended += (earlier + s_upto[32 * w + lane]) * per_row <= at.at;
+                earlier += s_scan[w];
+            }
+            ended = __reduce_add_sync(0xffffffffu, ended);
+            at.row = ended * chunk;
+            at.before = ended ? s_upto[ended - 1] : 0;
 #pragma unroll
-        for (int w = 0; w < WARPS - 1; ++w)
-            if (w < (ended - 1) >> 5) at.before += s_scan[w];
-        for (;; ++at.row) {
-            n = units_of(p, row_keys(p, at.row, false));
-            if (at.at < (at.before + n) * per_row) break;
-            at.before += n;
+            for (int w = 0; w < WARPS - 1; ++w)
+                if (w < (ended - 1) >> 5) at.before += s_scan[w];
+            for (;; ++at.row) {
+                n = units_of(p, row_keys(p, at.row, false));
+                if (at.at < (at.before + n) * per_row) break;
+                at.before += n;
+            }
         }
         if (c < 2) {
             const int s = at.before * per_row;
