@@ -432,7 +432,7 @@ beam_select_kernel(const SelectParams p) {
 // Runs that a beam's logits are cut into: one wave of four blocks an SM, no run
 // under 16 logits a thread, and the group's keys in the join's shared memory.
 int select_splits(int64_t rows, int beams, int64_t vocab, int n_out) {
-    const int64_t tiles = vocab / (16 * THREADS);
+    const int64_t tiles = (vocab + 16 * THREADS - 1) / (16 * THREADS);
     int64_t splits = 592 / rows;
     splits = splits < tiles ? splits : tiles;
     const int64_t most = JOIN_BYTES / 8 / ((int64_t)beams * (n_out + 1));

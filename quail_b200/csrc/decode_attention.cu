@@ -897,7 +897,7 @@ decode_attention_kernel(const Params p) {
                 const float m = in ? __ldcg(&part.m[head]) : NEG_INF;
                 const float l = in ? __ldcg(&part.l[head]) : 0.0f;
                 const float mv = in ? __ldcg(&part.mv[head]) : NEG_INF;
-                constexpr int BATCH = 16;   // parts whose columns are in flight together
+                constexpr int BATCH = 24;   // parts whose columns are in flight together
                 float4 o[BATCH];
                 auto fetch = [&](int i) {
 #pragma unroll
