@@ -865,15 +865,15 @@ decode_attention_kernel(const Params p) {
     if (!open) return;
 
     // ---- the parts that blocks share: the last to arrive joins them
-    __syncthreads();
     auto sharers = [&](const Slot<D>& slot, int& first, int& last) {   // the cuts inside the item
         first = cuts.from(slot.start + MIN_UNITS);
         last = cuts.from(slot.start + slot.n - MIN_UNITS + 1) - 1;
     };
-    if (tid < __popc(open)) {
-        const uint32_t which = tid == 0 ? open : open & (open - 1);
-        int first, last;
-        sharers(slots[__ffs(which) - 1], first, last);
+    const bool counts = tid < __popc(open);
+    int first = 0, last = 0;
+    if (counts) sharers(slots[__ffs(tid == 0 ? open : open & (open - 1)) - 1], first, last);
+    __syncthreads();
+    if (counts) {
         __threadfence();   // the block's parts, before the count
         const uint32_t others = atomicAdd(p.arrived + first, 1u);
         const bool all = others == (uint32_t)(last - first + 1);
@@ -886,7 +886,6 @@ decode_attention_kernel(const Params p) {
     for (int k = 0; which; ++k, which &= which - 1) {
         if (!s_joins[k]) continue;
         const Slot<D>& slot = slots[__ffs(which) - 1];
-        int first, last;
         sharers(slot, first, last);
         for (int head = warp; head < HEADS; head += WARPS) {
             Joined<FP8> j;
@@ -897,7 +896,8 @@ decode_attention_kernel(const Params p) {
                 const float m = in ? __ldcg(&part.m[head]) : NEG_INF;
                 const float l = in ? __ldcg(&part.l[head]) : 0.0f;
                 const float mv = in ? __ldcg(&part.mv[head]) : NEG_INF;
-                constexpr int BATCH = 24;   // parts whose columns are in flight together
+                constexpr int BATCH = 16;   // parts whose columns are in flight together
+                static_assert(32 % BATCH == 0, "a batch lies within the lanes' 32 parts");
                 float4 o[BATCH];
                 auto fetch = [&](int i) {
 #pragma unroll

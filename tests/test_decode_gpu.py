@@ -303,6 +303,17 @@ def test_decode_attention_lengths(dev, lengths, quant):
 
 
 @pytest.mark.parametrize("quant", [False, True])
+@pytest.mark.parametrize("n_q,d,lengths", [(8, 128, [40000]), (9, 64, [21000, 5]),
+                                           (3, 128, [600, 7000, 129] * 9)])
+def test_decode_attention_items_that_many_blocks_share(dev, n_q, d, lengths, quant):
+    """One KV head: a long row's parts come from every block."""
+    case = Case(dev, n_q, 1, d, lengths, quant=quant, seed=n_q)
+    out, lse = decode.decode_attention(case.q, case.kv, case.table, case.used, with_lse=True)
+    assert status() == 0
+    case.check(out, lse)
+
+
+@pytest.mark.parametrize("quant", [False, True])
 def test_decode_attention_sharp_and_flat_rows(dev, quant):
     """Keys that raise the running maximum at each step, one key far above the
     rest at either end, and products that are all equal."""
