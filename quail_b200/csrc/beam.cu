@@ -386,7 +386,28 @@ beam_select_kernel(const SelectParams p) {
                 sum += sums[i].x > -INFINITY ? sums[i].y * exp_approx(sums[i].x - m) : sums[i].y;
             sum = warp_sum(sum);
             if (lane == 0) s_lse[b] = m + logf(sum);
+        } else if (p.splits > 1 && list <= 96) {
+            // few keys: the place of each is the number above it
+            uint64_t* keys = s_lists + b * list;
+            uint64_t mine[3];
+            int place[3] = {n_out, n_out, n_out};
+#pragma unroll
+            for (int c = 0; c < 3; ++c) {
+                mine[c] = lane + 32 * c < list ? keys[lane + 32 * c] : 0;
+                if (lane + 32 * c < list) place[c] = 0;
+            }
+#pragma unroll 4
+            for (int j = 0; j < list; ++j) {
+                const uint64_t other = keys[j];
+#pragma unroll
+                for (int c = 0; c < 3; ++c) place[c] += other > mine[c];
+            }
+            __syncwarp();
+#pragma unroll
+            for (int c = 0; c < 3; ++c)
+                if (place[c] < n_out) keys[place[c]] = mine[c];
         } else if (p.splits > 1) {
+            // many: the best that is left, n_out times
             uint64_t* keys = s_lists + b * list;
             uint64_t limit = ~0ull, chosen = 0;   // of rank `lane`
             for (int r = 0; r < n_out; ++r) {
@@ -403,28 +424,46 @@ beam_select_kernel(const SelectParams p) {
         }
     }
     __syncthreads();
-    if (warp != 0) return;
-    // a beam a lane: its next offer
-    const bool live = lane < p.beams;
-    const bool done = live && p.finished && p.finished[row0 + lane];
-    const float score = live ? p.scores[row0 + lane] : 0.0f;
-    int rank = 0;
-    auto offer = [&]() -> uint64_t {
-        if (!live || rank == n_out) return 0;
-        float s = rank ? -INFINITY : score;
-        if (!done) s = score + (key_value(s_lists[lane * list + rank]) - s_lse[lane]);
-        return offer_key(s, lane * n_out + rank);
+    // a thread's beam (a beam a lane for many offers, below)
+    const int offers = p.beams * n_out;
+    const bool few = offers <= THREADS;
+    const int b = few ? tid / n_out : lane;
+    const bool live = few ? tid < offers : warp == 0 && lane < p.beams;
+    const bool done = live && p.finished && p.finished[row0 + b];
+    const float score = live ? p.scores[row0 + b] : 0.0f;
+    auto offer = [&](int rank) {
+        float s = rank ? -INFINITY : score;   // a finished beam's: itself
+        if (!done) s = score + (key_value(s_lists[b * list + rank]) - s_lse[b]);
+        return offer_key(s, b * n_out + rank);
     };
-    uint64_t mine = offer();
+    auto write = [&](int place, uint64_t key, int rank) {
+        const int64_t at = group * n_out + place;
+        p.scores_out[at] = key_value(key);
+        p.parent_out[at] = b;
+        p.token_out[at] = done ? p.pad : (int64_t)key_index(s_lists[b * list + rank]);
+    };
+    if (few) {
+        // an offer a thread; its place is the number above it (s_key is free)
+        const int rank = tid - b * n_out;
+        const uint64_t mine = live ? offer(rank) : 0;
+        if (live) s_key[tid] = mine;
+        __syncthreads();
+        if (!live) return;
+        int place = 0;
+#pragma unroll 8
+        for (int j = 0; j < offers; ++j) place += s_key[j] > mine;
+        if (place < n_out) write(place, mine, rank);
+        return;
+    }
+    if (warp != 0) return;
+    // a beam's next offer a lane; the best of these, n_out times
+    int rank = 0;
+    uint64_t mine = live ? offer(0) : 0;
     for (int r = 0; r < n_out; ++r) {
         const uint64_t best = warp_max64(mine);
         if (mine == best) {   // (one lane: keys differ)
-            const int64_t at = group * n_out + r;
-            p.scores_out[at] = key_value(best);
-            p.parent_out[at] = lane;
-            p.token_out[at] = done ? p.pad : (int64_t)key_index(s_lists[lane * list + rank]);
-            ++rank;
-            mine = offer();
+            write(r, best, rank);
+            mine = ++rank < n_out ? offer(rank) : 0;
         }
     }
 }

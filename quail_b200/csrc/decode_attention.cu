@@ -41,7 +41,11 @@ using namespace qb;
 constexpr int HEADS = 8;      // query heads of an item: the MMA's N
 constexpr int UNIT_SHIFT = 4; // a unit of work: 16 keys
 constexpr int MIN_UNITS = 8;          // a block's least part of an item that is cut
-constexpr int WHOLE_UNITS = 16;       // items up to this long are not cut
+// Items up to WHOLE_UNITS are not cut, nor, where blocks have fewer than
+// SHORT_UNITS each, items up to that: a cut costs a join through the workspace,
+// about 3 us, and saves its blocks' steps (one row of 300 tokens, 8 KV heads:
+// 10.1 us cut, 8.0 whole; at 32 units some 10 us cases take 13).
+constexpr int WHOLE_UNITS = 16, SHORT_UNITS = 28;
 
 // Warps of a block, one block an SM.
 template <bool FP8>
@@ -122,9 +126,10 @@ struct Cuts {
     }
 };
 
-// The cut x moved off short items and slivers, within the item [s, s + n)
-__device__ __forceinline__ int settle(int x, int s, int n) {
-    if (n <= WHOLE_UNITS || x - s < MIN_UNITS) return s;
+// The cut x moved off items of up to `whole` units and slivers, within the item
+// [s, s + n)
+__device__ __forceinline__ int settle(int x, int s, int n, int whole) {
+    if (n <= whole || x - s < MIN_UNITS) return s;
     return s + n - x < MIN_UNITS ? s + n : x;
 }
 
@@ -730,6 +735,7 @@ decode_attention_kernel(const Params p) {
     // places of its two cuts and of the warp's first unit. The threads whose
     // rows end at x or before are counted, then the next one's rows walked.
     const Cuts cuts(total, blocks);
+    const int whole_units = cuts.base < SHORT_UNITS ? SHORT_UNITS : WHOLE_UNITS;
     int lo = 0, hi = total, end = total, n = 0;
     Place at = {0, 0, 0};
 #pragma unroll 1
@@ -768,7 +774,7 @@ decode_attention_kernel(const Params p) {
         }
         if (c < 2) {
             const int s = at.before * per_row;
-            (c ? hi : lo) = settle(at.at, s + (at.at - s) / n * n, n);
+            (c ? hi : lo) = settle(at.at, s + (at.at - s) / n * n, n, whole_units);
         }
     }
 
