@@ -987,7 +987,7 @@ extern "C" int qb_decode_attention(const void* q, int64_t q_ld, int64_t rows, in
     if (q_ld < width || q_ld % 8 || !aligned(q, 16))
         return invalid("qb_decode_attention: q needs 16-byte alignment and q_ld a multiple of 8 "
                        "that covers the heads");
-    if (!out && !q_out) return invalid("qb_decode_attention: no output");
+    if (rows > 0 && !out && !q_out) return invalid("qb_decode_attention: no output");
     if (out && (out_ld < width || out_ld % 4 || !aligned(out, 8)))
         return invalid("qb_decode_attention: out needs 8-byte alignment and out_ld a multiple "
                        "of 4 that covers the heads");

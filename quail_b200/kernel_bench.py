@@ -6,7 +6,8 @@ events on the launching stream, and prints one JSON line: mean ms per
 launch, the algorithmic bytes or FLOPs of one launch and the achieved rate
 against the measured peaks (MEASURED_PEAKS.json beside the repository
 root, when present). Inputs are random device tensors of the Qwen3-4B
-config-1 shapes; they exist only to be read, so values do not matter.
+config-1 shapes; they exist only to be read, so values do not matter (of the
+beams' logits the order does: it is random).
 
 The same command with ``--warmup 0 --iters 1..3`` is the small case that
 a profiler capture of one kernel runs on.
@@ -22,6 +23,12 @@ Ops:
   norm       qb_add_rmsnorm_quant on (rows, hidden)
   rope       qb_qknorm_rope with the fused KV append on rows
   attention  qb_tree_attention on one packed config-1 chunk (--budget tokens)
+  decode     qb_decode_attention: --rows rows of --keys keys each, 32 query
+             heads over 8 KV heads of 128, bf16 or (--kv fp8) 8-bit pools
+  kv_quant   qb_kv_quant_write, and qb_kv_quant_read beside it, of --rows rows
+             (8 heads of 128)
+  beam       qb_beam_select over --rows beams in groups of --beams, vocabulary
+             151,936, bf16 logits
 """
 
 import argparse
@@ -302,10 +309,71 @@ def op_attention(torch, args):
             "bound": "tensor (bf16)", "algorithmic": flops, "pairs": pairs}
 
 
+def op_decode(torch, args):
+    """Attention of one new token per row, as a layer of a decode step."""
+    from quail_b200 import decode
+    from quail_b200.model import QWEN3_4B as cfg
+    rows, keys, page = args.rows, args.keys, 16
+    per = -(-keys // page)
+    ids = torch.randperm(rows * per, device="cuda").to(torch.int32)
+    table = ids.view(rows, per)
+    used = torch.full((rows,), keys, dtype=torch.int32, device="cuda")
+    q = torch.randn(rows, cfg.n_q, cfg.head_dim, device="cuda").to(torch.bfloat16)
+    shape = (rows * per * page, cfg.n_kv, cfg.head_dim)
+    if args.kv == "fp8":
+        quant = decode.QuantKV(1, rows * per, page, cfg.n_kv, cfg.head_dim)
+        quant.codes.view(torch.uint8).random_(0, 120)
+        quant.scales.random_(118, 122)
+        kv, row_bytes = quant.layer_kv(0), 2 * cfg.n_kv * (cfg.head_dim + 1)
+    else:
+        kv = tuple(torch.randn(shape, dtype=torch.bfloat16, device="cuda") for _ in range(2))
+        row_bytes = 4 * cfg.n_kv * cfg.head_dim
+
+    def launch():
+        decode.decode_attention(q, kv, table, used)
+    ms = time_launches(torch, launch, args.warmup, args.iters)
+    nbytes = rows * keys * row_bytes + 4 * q.numel()
+    return {"rows": rows, "keys": keys, "kv": args.kv, "ms": ms, "gbs": nbytes / ms / 1e6,
+            "bound": "hbm", "algorithmic": nbytes}
+
+
+def op_kv_quant(torch, args):
+    """A layer's K and V rows into the 8-bit cache, and back."""
+    from quail_b200 import decode
+    from quail_b200.model import QWEN3_4B as cfg
+    rows = args.rows
+    k, v = (torch.randn(rows, cfg.n_kv, cfg.head_dim, device="cuda").to(torch.bfloat16)
+            for _ in range(2))
+    kv = decode.QuantKV(1, -(-rows // 16), 16, cfg.n_kv, cfg.head_dim).layer_kv(0)
+    dst = torch.randperm(rows, device="cuda")
+    ms = time_launches(torch, lambda: decode.kv_quant_write(k, v, kv, dst), args.warmup,
+                       args.iters)
+    ms_read = time_launches(torch, lambda: decode.kv_quant_read(kv, dst, out=(k, v)),
+                            args.warmup, args.iters)
+    nbytes = rows * 2 * cfg.n_kv * (3 * cfg.head_dim + 1)
+    return {"rows": rows, "ms": ms, "ms_read": ms_read, "gbs": nbytes / ms / 1e6, "bound": "hbm",
+            "algorithmic": nbytes}
+
+
+def op_beam(torch, args):
+    """One choice over beams and vocabulary."""
+    from quail_b200 import decode
+    from quail_b200.model import QWEN3_4B as cfg
+    groups = args.rows // args.beams
+    rows = groups * args.beams
+    logits = (3 * torch.randn(rows, cfg.vocab, device="cuda")).to(torch.bfloat16)
+    scores = torch.randn(groups, args.beams, device="cuda")
+    ms = time_launches(torch, lambda: decode.beam_select(logits, scores), args.warmup,
+                       args.iters)
+    nbytes = rows * cfg.vocab * 2
+    return {"groups": groups, "beams": args.beams, "ms": ms, "gbs": nbytes / ms / 1e6,
+            "bound": "hbm", "algorithmic": nbytes}
+
+
 def main(argv=None):
     p = argparse.ArgumentParser(description=__doc__.split("\n")[0])
     p.add_argument("op", choices=["gemm", "gate_up", "qkv_rope", "layer", "silu", "norm",
-                                  "rope", "attention"])
+                                  "rope", "attention", "decode", "kv_quant", "beam"])
     p.add_argument("--m", type=int, default=65536)
     p.add_argument("--n", type=int, default=6144)
     p.add_argument("--k", type=int, default=2560)
@@ -315,6 +383,9 @@ def main(argv=None):
     p.add_argument("--budget", type=int, default=110376)
     p.add_argument("--doc-rows", type=int, default=2000)
     p.add_argument("--pages", type=int, default=16384)
+    p.add_argument("--keys", type=int, default=4096)
+    p.add_argument("--kv", choices=["bf16", "fp8"], default="bf16")
+    p.add_argument("--beams", type=int, default=8)
     p.add_argument("--warmup", type=int, default=3)
     p.add_argument("--iters", type=int, default=20)
     p.add_argument("--ue8m0", action="store_true",

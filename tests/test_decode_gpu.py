@@ -476,6 +476,22 @@ def test_decode_attention_on_another_stream_and_in_a_graph(dev):
     assert status() == 0
 
 
+def test_no_rows(dev):
+    """Zero rows and groups: empty results, nothing launched on them."""
+    kv = (torch.zeros(32, 2, 128, dtype=torch.bfloat16, device=dev),) * 2
+    q = torch.zeros(0, 8, 128, dtype=torch.bfloat16, device=dev)
+    table = torch.zeros(0, 3, dtype=torch.int32, device=dev)
+    out, lse = decode.decode_attention(q, kv, table, table[:, 0].contiguous(), with_lse=True)
+    assert out.shape == (0, 8, 128) and lse.shape == (0, 8)
+    got = decode.beam_select(torch.zeros(0, 50, device=dev), torch.zeros(0, 4, device=dev))
+    assert [t.shape for t in got] == [(0, 4)] * 3
+    pool = torch.zeros(1, 2, 32, 1, 64, dtype=torch.bfloat16, device=dev)
+    parents = torch.zeros(0, 4, dtype=torch.int32, device=dev)
+    table, rows = decode.beam_reorder((pool,), parents, parents[:, 0].contiguous(), table)
+    assert table.shape == (0, 3) and rows.shape == (0,)
+    assert status() == 0
+
+
 def test_decode_attention_repeats_bit_for_bit(dev):
     case = Case(dev, 32, 8, 128, [9000, 100, 2500, 1], seed=12)
     first = decode.decode_attention(case.q, case.kv, case.table, case.used, with_lse=True)
