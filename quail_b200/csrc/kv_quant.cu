@@ -29,17 +29,24 @@ __device__ __forceinline__ float e8m0_float(uint32_t b) {
     return __uint_as_float(b ? b << 23 : 0x00400000u);
 }
 
+// the larger of two pairs of unsigned 16-bit numbers
+__device__ __forceinline__ uint32_t max_u16x2(uint32_t a, uint32_t b) {
+    uint32_t r;
+    asm("max.u16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
+    return r;
+}
+
 // Quantises 8 values of a head held by LANES consecutive lanes (8 each).
 template <int LANES>
 __device__ __forceinline__ uint2 quant8(const uint4& raw, uint32_t& byte) {
     // the largest magnitude by its bits, two bf16 at a time; a NaN is above
     // every infinity and so is kept
     constexpr uint32_t ABS = 0x7FFF7FFFu;
-    uint32_t top = __vmaxu2(__vmaxu2(raw.x & ABS, raw.y & ABS),
-                            __vmaxu2(raw.z & ABS, raw.w & ABS));
+    uint32_t top = max_u16x2(max_u16x2(raw.x & ABS, raw.y & ABS),
+                            max_u16x2(raw.z & ABS, raw.w & ABS));
 #pragma unroll
     for (int o = LANES / 2; o > 0; o >>= 1)
-        top = __vmaxu2(top, __shfl_xor_sync(0xffffffffu, top, o));
+        top = max_u16x2(top, __shfl_xor_sync(0xffffffffu, top, o));
     top = max(top << 16, top & 0xFFFF0000u);
     if (top >= 0x7F800000u) {
         byte = 255u;
@@ -64,6 +71,26 @@ __device__ __forceinline__ uint2 quant8(const uint4& raw, uint32_t& byte) {
     return make_uint2(c[0] | (c[1] << 16), c[2] | (c[3] << 16));
 }
 
+// The pieces of a thread, THREADS apart: each one's row in the block and place
+// in the row, without a division a piece.
+struct Pieces {
+    int row, at, step_row, step_at;
+    __device__ __forceinline__ Pieces(int first, int chunks) {
+        row = first / chunks;
+        at = first - row * chunks;
+        step_row = THREADS / chunks;
+        step_at = THREADS - step_row * chunks;
+    }
+    __device__ __forceinline__ void advance(int chunks) {
+        row += step_row;
+        at += step_at;
+        if (at >= chunks) {
+            at -= chunks;
+            ++row;
+        }
+    }
+};
+
 // A block takes `per_block` rows, each of `chunks` pieces for K and V; a
 // thread's pieces are THREADS apart, so LANES neighbouring lanes hold a head.
 template <int D>
@@ -77,21 +104,23 @@ kv_quant_write_kernel(const bf16* __restrict__ k, const bf16* __restrict__ v, in
     constexpr int LANES = D / 8;
     const int64_t row0 = (int64_t)blockIdx.x * per_block;
     const int all = (int)min((int64_t)per_block, n - row0) * chunks;
+    Pieces next(threadIdx.x, chunks);
     for (int base = threadIdx.x & ~31; base < all; base += THREADS * BATCH) {
         uint4 raw[2][BATCH];
         int64_t to[BATCH];   // the destination row, -1: none
         int at[BATCH];
 #pragma unroll
         for (int j = 0; j < BATCH; ++j) {
-            const int i = base + THREADS * j + (threadIdx.x & 31);
+            const int64_t row = row0 + next.row;
+            const bool in = base + THREADS * j + (int)(threadIdx.x & 31) < all;
+            at[j] = next.at;
+            next.advance(chunks);
             to[j] = -1;
             raw[0][j] = raw[1][j] = make_uint4(0, 0, 0, 0);
-            if (i >= all) continue;
-            const int r = i / chunks;
-            at[j] = i - r * chunks;
-            const int64_t d = dst[row0 + r];
+            if (!in) continue;
+            const int64_t d = dst[row];
             if (d < 0) continue;   // a row that is not kept
-            const int64_t s = src ? src[row0 + r] : row0 + r;
+            const int64_t s = src ? src[row] : row;
             if (d >= pool_rows || s < 0 || s >= src_rows) {
                 if (at[j] == 0) atomicOr(status, STATUS_BAD_INDEX);
                 continue;
@@ -107,12 +136,12 @@ kv_quant_write_kernel(const bf16* __restrict__ k, const bf16* __restrict__ v, in
             const uint2 kq = quant8<LANES>(raw[0][j], kb);
             const uint2 vq = quant8<LANES>(raw[1][j], vb);
             if (to[j] < 0) continue;
-            const int64_t place = to[j] * n_kv * D + at[j] * 8;
+            const int64_t head = to[j] * n_kv, place = head * D + at[j] * 8;
             *reinterpret_cast<uint2*>(k_codes + place) = kq;
             *reinterpret_cast<uint2*>(v_codes + place) = vq;
             if (at[j] % LANES == 0) {
-                k_scale[to[j] * n_kv + at[j] / LANES] = (uint8_t)kb;
-                v_scale[to[j] * n_kv + at[j] / LANES] = (uint8_t)vb;
+                k_scale[head + at[j] / LANES] = (uint8_t)kb;
+                v_scale[head + at[j] / LANES] = (uint8_t)vb;
             }
         }
     }
@@ -139,6 +168,7 @@ kv_quant_read_kernel(const uint8_t* __restrict__ k_codes, const uint8_t* __restr
     constexpr int LANES = D / 8;
     const int64_t row0 = (int64_t)blockIdx.x * per_block;
     const int all = (int)min((int64_t)per_block, n - row0) * chunks;
+    Pieces next(threadIdx.x, chunks);
     for (int base = threadIdx.x; base < all; base += THREADS * BATCH) {
         uint2 codes[2][BATCH];
         uint32_t bytes[2][BATCH];
@@ -146,16 +176,16 @@ kv_quant_read_kernel(const uint8_t* __restrict__ k_codes, const uint8_t* __restr
         int at[BATCH];
 #pragma unroll
         for (int j = 0; j < BATCH; ++j) {
-            const int i = base + THREADS * j;
+            const int64_t row = row0 + next.row;
+            at[j] = next.at;
+            next.advance(chunks);
             to[j] = -1;
             codes[0][j] = codes[1][j] = make_uint2(0, 0);
             bytes[0][j] = bytes[1][j] = 127u;
-            if (i >= all) continue;
-            const int r = i / chunks;
-            at[j] = i - r * chunks;
-            const int64_t d = dst ? dst[row0 + r] : row0 + r;
+            if (base + THREADS * j >= all) continue;
+            const int64_t d = dst ? dst[row] : row;
             if (d < 0) continue;
-            const int64_t s = src[row0 + r];
+            const int64_t s = src[row];
             if (d >= out_rows || s < 0 || s >= pool_rows) {
                 if (at[j] == 0) atomicOr(status, STATUS_BAD_INDEX);
                 to[j] = d < out_rows ? d : -1;   // zeros for a bad source
