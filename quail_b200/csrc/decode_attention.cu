@@ -17,7 +17,17 @@
 // smallest tile has 64 rows and wants its operands in shared memory by way of
 // descriptors; here a lane's 16-byte global loads are the operand fragments
 // themselves (the inner dimension's order is free, so each lane takes the
-// columns that it loaded), and nothing is staged.
+// columns that it loaded), and nothing is staged. (Staged through a ring of
+// cp.async copies, two steps ahead, 128 rows of 4k to 16k keys took 1,083 us
+// against 693.)
+//
+// Measured on a B200 (copy rate 6.55 TB/s), 32 query heads over 8 KV heads of
+// 128: 128 rows of 8,192 keys 642 us, 6.69 TB/s (8 bit: 402 us, 5.39 TB/s);
+// 256 rows of 96 to 2,112 keys 118 us, 88% of the copy rate; one row of 40,960
+// keys 37 us, 70%, a quarter of it the start and the join; one row of 37 keys
+// 5.3 us. The 8-bit cache is slower by the byte: its 128-byte rows, 1 KB apart,
+// reach 81% where one KV head's rows lie together at 89%, and a step's 574
+// instructions a warp leave two warps a scheduler little to hide latency with.
 //
 // Split and join. The rows' lengths are known on the device only (a captured
 // launch serves every step), so the blocks share the work there: an item is
@@ -38,20 +48,25 @@ namespace {
 
 using namespace qb;
 
-constexpr int HEADS = 8;      // query heads of an item: the MMA's N
-constexpr int UNIT_SHIFT = 4; // a unit of work: 16 keys
-constexpr int MIN_UNITS = 8;          // a block's least part of an item that is cut
+constexpr int HEADS = 8;        // query heads of an item: the MMA's N
+constexpr int UNIT_SHIFT = 4;   // a unit of work: 16 keys
+constexpr int MIN_UNITS = 8;    // a block's least part of an item that is cut
 // Items up to WHOLE_UNITS are not cut, nor, where blocks have fewer than
 // SHORT_UNITS each, items up to that: a cut costs a join through the workspace,
 // about 3 us, and saves its blocks' steps (one row of 300 tokens, 8 KV heads:
 // 10.1 us cut, 8.0 whole; at 32 units some 10 us cases take 13).
 constexpr int WHOLE_UNITS = 16, SHORT_UNITS = 28;
 
-// Warps of a block, one block an SM.
+// Warps of a block, one block an SM: as many as leave the registers for the
+// next step's K and V beside this one's. bf16: 10 (168 registers) 674 us for 128
+// rows of 4k to 16k keys, 116 for 256 rows of 96 to 2,112, 37.6 for one of 40,960;
+// 8 692, 122 and 38.0; 12 666, 118 and 39.5; 16 spills (867). 8 bit: 8 (255
+// registers) 60 us for 16 long rows, 10 spills (72).
 template <bool FP8>
 constexpr int warps() {
     return FP8 ? 8 : 10;
 }
+
 constexpr float LN2 = 0.693147180559945309f;
 constexpr float LOG2E = 1.44269504088896341f;
 
@@ -303,7 +318,8 @@ __device__ __forceinline__ void attend(const Params& p, Slot<D>& slot, int row, 
 #pragma unroll
         for (int j = 0; j < 4; ++j) o[i][j] = 0.0f;
 
-    // A step: 16 keys of 128 bf16, else 32. The pipeline: while a step is
+    // A step: 16 keys of 128 bf16, else 32 (8 bit, D = 128: 59.4 us for 16 long
+    // rows against 61.5 with 16 keys and 12 warps). The pipeline: while a step is
     // computed, the next one's K (as soon as S has consumed the registers), V
     // (after the second product) and, one further, the page ids are on their
     // way. Keys past the end are taken as the last one, with a weight of zero.
@@ -433,7 +449,9 @@ __device__ __forceinline__ void attend(const Params& p, Slot<D>& slot, int row, 
             }
         }
         const uint32_t now_lost = lost;
-        load_k(key0 + STEP);   // (past the end: the last key again)
+        // (past the end: the last key again; behind a branch these loads are not
+        // moved up: 740 us against 670 for 128 long rows)
+        load_k(key0 + STEP);
         // x, and y = x and the value's exponent: [2 * half + head]
         float x[UNITS][4], y[UNITS][4];
 #pragma unroll
@@ -684,7 +702,8 @@ decode_attention_kernel(const Params p) {
     const int per_row = p.n_kv * p.tiles;   // items of a row
 
     // ---- a scan over the rows' units: up to 32 rows by every warp for itself, a
-    // row a lane; more by the block, `chunk` rows a thread
+    // row a lane (one short row 5.3 us against 5.9); more by the block, `chunk`
+    // rows a thread
     const bool few = p.rows <= 32;
     const int chunk = few ? 1 : (p.rows + THREADS - 1) / THREADS;
     const int r0 = min((few ? lane : tid) * chunk, p.rows), r1 = min(r0 + chunk, p.rows);
