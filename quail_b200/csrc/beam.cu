@@ -11,7 +11,7 @@
 // each block a run of one beam's; a logit costs a maximum, an exponential and
 // an addition in fp32. A block keeps its n_out best so far as sorted keys
 // (value, lower token first), and a bar: first the n_out-th largest of the
-// first tile's maxima of 8 threads, later the last of the best. Logits that
+// first tile's 32 groups' maxima, later the last of the best. Logits that
 // pass are put on a list, without a barrier, and the list is ranked after 9,
 // 81, ... tiles and at the end: of a run in no order about 8 n_out pass between. Where more pass than the list
 // holds (logits that rise along the run, or many equal ones), the run is gone
@@ -19,11 +19,11 @@
 // putting its best forward, and again, until none does. The block that completes its group (a counter) joins the runs and the beams, in an
 // order that does not depend on who came last.
 //
-// Measured on a B200, vocabulary 151,936: 16 groups of 8 beams, bf16 22 us (27%
-// of the copy rate), f32 27 us (44%); 4 beams of one group 8.5 us. Of the 22 us,
-// the exponentials alone need 4.4 (16 a clock an SM), reading 6; a block's start,
-// its ranking and the join of the group take the latency of about ten dependent
-// steps, and without exponentials and list it still takes 16.
+// Measured on a B200, vocabulary 151,936: 16 groups of 8 beams, bf16 19 us (31%
+// of the copy rate), f32 24 us (49%); 4 beams of one group 8.4 us. Of the 19 us,
+// the exponentials alone need 4.4 (16 a clock an SM) and reading 6; a block's
+// start, its ranking and the join of the group take the latency of about ten
+// dependent steps.
 #include "common.cuh"
 
 namespace {
@@ -33,9 +33,12 @@ using namespace qb;
 constexpr int MAX_BEAMS = 32;
 constexpr int MAX_OUT = 32;
 constexpr int MAX_ROWS = 65535;        // groups * beams
-constexpr int THREADS = 256;
 constexpr int VECTORS = 4;             // 16-byte vectors of a thread in a tile
-constexpr int LIST = 2 * THREADS - MAX_OUT;   // keys; with the best, two a thread
+// Keys on the list: at least one a thread, and two a thread with the best.
+template <int THREADS>
+constexpr int list_keys() {
+    return THREADS > 512 ? THREADS : 512 - MAX_OUT;
+}
 constexpr int JOIN_BYTES = 40 * 1024;  // a group's keys in the join
 constexpr float LOG2E = 1.44269504088896341f;
 
@@ -140,12 +143,14 @@ struct SelectParams {
 };
 
 // Block (split, row): a run of one beam's logits.
-template <typename T>
-__global__ void __launch_bounds__(THREADS, 4)
+template <typename T, int THREADS>
+__global__ void __launch_bounds__(THREADS, 1024 / THREADS)
 beam_select_kernel(const SelectParams p) {
-    constexpr int VE = Vector<T>::N, TILE = VECTORS * VE * THREADS;
+    constexpr int VE = Vector<T>::N, TILE = VECTORS * VE * THREADS, LIST = list_keys<THREADS>();
+    constexpr int GROUP = THREADS / 32;   // threads of one of 32 groups
+    static_assert(MAX_OUT + LIST <= 2 * THREADS, "rank() holds two keys a thread");
     __shared__ uint64_t s_key[MAX_OUT + LIST];   // the best so far, in order; the list
-    __shared__ __align__(16) uint32_t s_group[THREADS / 8];
+    __shared__ __align__(16) uint32_t s_group[32];
     __shared__ uint32_t s_new;
     __shared__ float s_m[THREADS / 32], s_s[THREADS / 32];
     __shared__ bool s_last;
@@ -262,9 +267,9 @@ beam_select_kernel(const SelectParams p) {
                 const bool some = at < v1 || single >= 0;
                 uint32_t mine = some ? order_key(top) : 0u;
 #pragma unroll
-                for (int o = 1; o < 8; o <<= 1)
+                for (int o = 1; o < GROUP; o <<= 1)
                     mine = max(mine, __shfl_xor_sync(0xffffffffu, mine, o));
-                if (lane % 8 == 0) s_group[tid / 8] = mine;
+                if (lane % GROUP == 0) s_group[tid / GROUP] = mine;
                 __syncthreads();
                 mine = s_group[lane];
                 int above = 0;
@@ -475,15 +480,25 @@ beam_select_kernel(const SelectParams p) {
     }
 }
 
-// Runs that a beam's logits are cut into: one wave of four blocks an SM, no run
-// under 16 logits a thread, and the group's keys in the join's shared memory.
-int select_splits(int64_t rows, int beams, int64_t vocab, int n_out) {
-    const int64_t tiles = (vocab + 16 * THREADS - 1) / (16 * THREADS);
+// How a call is cut: threads of a block, and runs of a beam's logits. Blocks of
+// 1,024 threads, one an SM, where they fill four fifths of the GPU with runs of
+// 16 logits a thread or more (one ranking and one list for four times the
+// logits: 16 groups of 8 beams in bf16 19 us against 22); else blocks of 256, four an
+// SM in one wave, no run under 16 logits a thread. The group's keys fit the
+// join's shared memory.
+struct Cut {
+    int threads, splits;
+};
+Cut cut_of(int64_t rows, int beams, int64_t vocab, int n_out) {
+    const int64_t most = JOIN_BYTES / 8 / ((int64_t)beams * (n_out + 1));
+    const int64_t wide = 148 / rows;
+    if (wide >= 1 && wide <= most && rows * wide >= 118 && vocab / wide >= 16 * 1024)
+        return {1024, (int)wide};
+    const int64_t tiles = (vocab + 16 * 256 - 1) / (16 * 256);
     int64_t splits = 592 / rows;
     splits = splits < tiles ? splits : tiles;
-    const int64_t most = JOIN_BYTES / 8 / ((int64_t)beams * (n_out + 1));
     splits = splits < most ? splits : most;
-    return splits < 1 ? 1 : (int)splits;
+    return {256, splits < 1 ? 1 : (int)splits};
 }
 
 // ---- reordering -------------------------------------------------------------
@@ -601,7 +616,7 @@ extern "C" int qb_beam_select_workspace(int64_t groups, int beams, int64_t vocab
     // the counters, always at the same place, then the runs' keys and sums
     *bytes = MAX_ROWS * 4 + 4;
     if (groups)
-        *bytes += groups * beams * select_splits(groups * beams, beams, vocab, n_out) *
+        *bytes += groups * beams * cut_of(groups * beams, beams, vocab, n_out).splits *
                   ((int64_t)n_out * 8 + 8);
     return QB_OK;
 }
@@ -635,7 +650,8 @@ extern "C" int qb_beam_select(const void* logits, int logits_bf16, int64_t logit
     p.vocab = vocab;
     p.beams = beams;
     p.n_out = n_out;
-    p.splits = select_splits(rows, beams, vocab, n_out);
+    const Cut cut = cut_of(rows, beams, vocab, n_out);
+    p.splits = cut.splits;
     p.scores = scores;
     p.finished = finished;
     p.pad = pad;
@@ -647,10 +663,11 @@ extern "C" int qb_beam_select(const void* logits, int logits_bf16, int64_t logit
     p.token_out = token_out;
     const dim3 grid((unsigned)p.splits, (unsigned)rows);
     const int bytes = beams * p.splits * (n_out + 1) * 8;
-    if (logits_bf16)
-        beam_select_kernel<bf16><<<grid, THREADS, bytes, (cudaStream_t)stream>>>(p);
-    else
-        beam_select_kernel<float><<<grid, THREADS, bytes, (cudaStream_t)stream>>>(p);
+    auto* kernel = logits_bf16 ? (cut.threads == 1024 ? beam_select_kernel<bf16, 1024>
+                                                      : beam_select_kernel<bf16, 256>)
+                               : (cut.threads == 1024 ? beam_select_kernel<float, 1024>
+                                                      : beam_select_kernel<float, 256>);
+    kernel<<<grid, cut.threads, bytes, (cudaStream_t)stream>>>(p);
     return launch_status(who);
 }
 

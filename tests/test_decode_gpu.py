@@ -633,6 +633,26 @@ def test_beam_select_adverse_orders(dev, kind, dtype):
 
 
 @pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("groups,beams,vocab,n_out", [(15, 8, 20000, 8), (4, 32, 17001, 32),
+                                                      (64, 1, 40001, 5), (37, 4, 16385, 3)])
+def test_beam_select_wide_blocks(dev, groups, beams, vocab, n_out, dtype):
+    """Enough rows of a long vocabulary for the wide blocks: random logits, and
+    for some rows the orders and masks that the list does not hold."""
+    g = torch.Generator(device=dev).manual_seed(groups + vocab)
+    logits = 3 * torch.randn(groups * beams, vocab, generator=g, device=dev)
+    logits[1] = torch.arange(vocab, device=dev) / 1000.0
+    logits[2] = -1.5
+    logits[3] = -math.inf
+    logits[4, 7::3000] = math.nan
+    logits[5] = -math.inf
+    logits[5, 11::4000] = 0.5
+    logits[6] = torch.arange(vocab, device=dev) // 100 % 5
+    logits = logits.to(dtype)
+    scores = -5 + torch.randn(groups, beams, generator=g, device=dev)
+    check_select(decode.beam_select(logits, scores, n_out=n_out), logits, scores)
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
 def test_beam_select_strided_rows(dev, dtype):
     """Rows at a stride that leaves them at every alignment."""
     g = torch.Generator(device=dev).manual_seed(3)
