@@ -195,8 +195,9 @@ beam_select_kernel(const SelectParams p) {
         };
         // the n_out best of those so far and `fresh` on the list, into their
         // places: a key's place is the number of keys above it, so the order of
-        // arrival does not matter (between barriers)
-        auto rank = [&](int fresh) {
+        // arrival does not matter (between barriers). `again`: the list is used
+        // again, so it is emptied, after every warp has read how long it was.
+        auto rank = [&](int fresh, bool again) {
             const int n = n_out + fresh;
             uint64_t mine[2];
             int place[2] = {n_out, n_out};
@@ -209,14 +210,14 @@ beam_select_kernel(const SelectParams p) {
                 for (int j = 0; j < n; ++j) above += s_key[j] > mine[c];
                 place[c] = above;
             }
-            if (n > 32)
+            if (again || n > 32)
                 __syncthreads();
             else
                 __syncwarp();   // one warp holds them all
 #pragma unroll
             for (int c = 0; c < 2; ++c)
                 if (place[c] < n_out) s_key[place[c]] = mine[c];
-            if (tid == 0) s_new = 0;
+            if (again && tid == 0) s_new = 0;
             __syncthreads();
             least = s_key[n_out - 1];
         };
@@ -307,7 +308,7 @@ beam_select_kernel(const SelectParams p) {
                 const int fresh = s_new;
                 over = fresh > LIST;
                 if (!over && fresh)
-                    rank(fresh);
+                    rank(fresh, true);
                 else
                     __syncthreads();   // s_new has been read
             }
@@ -337,11 +338,11 @@ beam_select_kernel(const SelectParams p) {
                     put_on_list(key);
                     if (key) limit = key;
                     __syncthreads();
-                    rank(put);
+                    rank(put, true);
                 }
             }
         } else if (fresh) {
-            rank(fresh);
+            rank(fresh, false);
         }
         // ---- the run's results
         float sum, second;

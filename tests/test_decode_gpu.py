@@ -652,6 +652,21 @@ def test_beam_select_wide_blocks(dev, groups, beams, vocab, n_out, dtype):
     check_select(decode.beam_select(logits, scores, n_out=n_out), logits, scores)
 
 
+@pytest.mark.parametrize("groups,beams,vocab,n_out", [
+    (1, 2, 300, 2), (1, 1, 9000, 1), (300, 2, 45000, 2), (1, 1, 148 * 150000, 1),
+    (60, 2, 300000, 1)])
+def test_beam_select_short_lists(dev, groups, beams, vocab, n_out):
+    """Lists that one warp ranks, within a run and at its end, call after call:
+    the same choice each time."""
+    g = torch.Generator(device=dev).manual_seed(groups + vocab)
+    logits = 3 * torch.randn(groups * beams, vocab, generator=g, device=dev)
+    scores = -5 + torch.randn(groups, beams, generator=g, device=dev)
+    got = [decode.beam_select(logits, scores, n_out=n_out) for _ in range(50)]
+    for other in got[1:]:
+        assert all(torch.equal(a, b) for a, b in zip(got[0], other))
+    check_select(got[0], logits, scores)
+
+
 @pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
 def test_beam_select_strided_rows(dev, dtype):
     """Rows at a stride that leaves them at every alignment."""
