@@ -679,10 +679,10 @@ extern "C" int qb_beam_reorder(const int32_t* parents, const int32_t* used, int6
                                int32_t* table_out, int64_t* next_row, void* stream) {
     const char* who = "qb_beam_reorder";
     if (beams <= 0 || beams > MAX_BEAMS) return invalid("qb_beam_reorder: 1 to 32 beams a group");
-    if (groups < 0 || groups * beams > 65535)
+    if (groups < 0 || groups > MAX_ROWS || groups * beams > MAX_ROWS)
         return invalid("qb_beam_reorder: 0 to 65,535 rows");
     if (page_tokens <= 0 || page_tokens > 1024 || n_pages <= 0 || table_width <= 0 ||
-        n_slabs < 0 || n_slabs > (1 << 20) || row_bytes > (1 << 20))
+        table_width > (1 << 30) || n_slabs < 0 || n_slabs > (1 << 20) || row_bytes > (1 << 20))
         return invalid("qb_beam_reorder: bad page, table, slab or row sizes");
     if (n_slabs > 0 && (!pool || row_bytes <= 0 || row_bytes % 16 || !aligned(pool, 16)))
         return invalid("qb_beam_reorder: pool rows must be multiples of 16 bytes, 16-byte aligned");

@@ -89,6 +89,7 @@ REORDER = dict(parents=OK, used=OK, groups=2, beams=4, table=OK, width=4, page=1
 
 @pytest.mark.parametrize("change,match", [
     (dict(beams=0), "beams"), (dict(groups=20000), "rows"), (dict(page=0), "page"),
+    (dict(groups=1 << 62), "rows"), (dict(width=(1 << 62) + 1), "table"),
     (dict(row_bytes=24), "multiples of 16"), (dict(pool=OFF), "aligned"),
     (dict(pool2=OK), "row_bytes2"), (dict(out=None), "NULL"), (dict(out=OK), "table_in")])
 def test_beam_reorder_refuses(change, match):
