@@ -433,8 +433,8 @@ int qb_beam_select_workspace(int64_t groups, int beams, int64_t vocab, int n_out
  * logits: f32 (or bf16 when logits_bf16) [groups * beams, vocab], rows
  * logits_ld apart; scores: f32 [groups, beams]; finished: u8 [groups, beams] or
  * NULL; scores_out: f32, parent_out: int32 (beam within the group), token_out:
- * int64, each [groups, n_out]. 1 to 32 beams and n_out, vocab >= n_out,
- * groups * beams <= 65,535. workspace: qb_beam_select_workspace bytes, zero
+ * int64, each [groups, n_out]. 1 to 32 beams and n_out, vocab from
+ * n_out to 2^30, groups * beams <= 65,535. workspace: qb_beam_select_workspace bytes, zero
  * before its first call (each call leaves its counters zero, at the same place
  * for all sizes); calls that may run at the same time need one each.
  */

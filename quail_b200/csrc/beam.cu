@@ -33,6 +33,7 @@ using namespace qb;
 constexpr int MAX_BEAMS = 32;
 constexpr int MAX_OUT = 32;
 constexpr int MAX_ROWS = 65535;        // groups * beams
+constexpr int64_t MAX_VOCAB = 1 << 30; // a place and a block's step past it fit 32 bits
 constexpr int VECTORS = 4;             // 16-byte vectors of a thread in a tile
 // Keys on the list: at least one a thread, and two a thread with the best.
 template <int THREADS>
@@ -612,7 +613,7 @@ extern "C" int qb_beam_select_workspace(int64_t groups, int beams, int64_t vocab
                                         int64_t* bytes) {
     if (!bytes || groups < 0 || beams <= 0 || beams > MAX_BEAMS || groups > MAX_ROWS ||
         groups * beams > MAX_ROWS || n_out <= 0 || n_out > MAX_OUT || vocab < n_out ||
-        vocab > 0x7fffffffLL)
+        vocab > MAX_VOCAB)
         return invalid("qb_beam_select_workspace: bad sizes");
     // the counters, always at the same place, then the runs' keys and sums
     *bytes = MAX_ROWS * 4 + 4;
@@ -631,9 +632,9 @@ extern "C" int qb_beam_select(const void* logits, int logits_bf16, int64_t logit
     if (beams <= 0 || beams > MAX_BEAMS || n_out <= 0 || n_out > MAX_OUT)
         return invalid("qb_beam_select: 1 to 32 beams and 1 to 32 outputs a group");
     if (groups < 0 || groups > MAX_ROWS || groups * beams > MAX_ROWS || vocab < n_out ||
-        vocab > 0x7fffffffLL || logits_ld < vocab)
-        return invalid("qb_beam_select: at most 65,535 rows, vocab must hold n_out tokens and "
-                       "logits_ld the vocab");
+        vocab > MAX_VOCAB || logits_ld < vocab)
+        return invalid("qb_beam_select: at most 65,535 rows and 2^30 tokens, vocab must hold n_out "
+                       "tokens and logits_ld the vocab");
     if (groups == 0) return QB_OK;
     if (!logits || !scores || !scores_out || !parent_out || !token_out)
         return invalid("qb_beam_select: NULL tensor");

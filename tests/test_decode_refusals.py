@@ -76,7 +76,8 @@ SELECT = dict(logits=OK, bf16=0, ld=100, groups=2, beams=4, vocab=100, scores=OK
 
 @pytest.mark.parametrize("change,match", [
     (dict(beams=33), "beams"), (dict(n_out=0), "outputs"), (dict(n_out=33), "outputs"),
-    (dict(vocab=3, ld=3), "vocab"), (dict(ld=99), "logits_ld"), (dict(logits=None), "NULL"),
+    (dict(vocab=3, ld=3), "vocab"), (dict(vocab=2**31 - 1, ld=2**31), "vocab"),
+    (dict(ld=99), "logits_ld"), (dict(logits=None), "NULL"),
     (dict(ws=None), "workspace"), (dict(ws_bytes=8), "workspace")])
 def test_beam_select_refuses(change, match):
     refused(match, "qb_beam_select", *dict(SELECT, **change).values())
