@@ -160,6 +160,7 @@ std::tuple<Tensor, Tensor> kv_quant_read(const Tensor& kc, const Tensor& vc, con
          "src must be a contiguous int64 vector as long as the rows");
     const int64_t n = src.size(0);
     need(out_k || !dst, who, "dst needs out");
+    need(out_k.has_value() == out_v.has_value(), who, "out is a pair of tensors");
     Tensor k, v;
     if (out_k) {
         k = *out_k;

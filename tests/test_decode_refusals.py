@@ -113,6 +113,9 @@ def test_python_refusals():
             decode.kv_quant_write(*args)
     with pytest.raises(ValueError, match="dst needs out"):
         decode.kv_quant_read(kv, dst, dst=dst)
+    for out in ((k, None), (None, k)):
+        with pytest.raises(ValueError, match="pair"):
+            decode.kv_quant_read(kv, dst, out=out)
     q, table = torch.zeros(3, 4, 128, **bf), torch.zeros(3, 2, dtype=torch.int32)
     used, pools = torch.zeros(3, dtype=torch.int32), (torch.zeros(32, 2, 128, **bf),) * 2
     for match, args in (
