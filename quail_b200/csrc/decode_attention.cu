@@ -38,7 +38,7 @@
 // heads, cut alike, where the SMs divide so (8 KV heads: 18 blocks each, 4 of 148
 // left over): blocks next to each other then walk the same keys of neighbouring
 // heads, whose short rows lie together in memory (64 rows of 4k to 16k keys, 8
-// KV heads: 185 us against 199, 8 bit 155 against 182; heads of 128, 8 bit: 217
+// KV heads: 181 us against 207, 8 bit 123 against 164; heads of 128, 8 bit: 217
 // both ways, bf16 690 us against 696). A warp walks
 // its range alone; items that lie within it are finished there, the parts of
 // the others (two a warp at most) meet in shared memory at the block's end,
@@ -67,10 +67,12 @@ constexpr int WHOLE_UNITS = 16, SHORT_UNITS = 28;
 // next step's K and V beside this one's. bf16: 10 (168 registers) 674 us for 128
 // rows of 4k to 16k keys, 116 for 256 rows of 96 to 2,112, 37.6 for one of 40,960;
 // 8 692, 122 and 38.0; 12 666, 118 and 39.5; 16 spills (867). 8 bit: 8 (255
-// registers) 60 us for 16 long rows, 10 spills (72).
-template <bool FP8>
+// registers) 60 us for 16 long rows, 10 spills (72). Heads of 64: 12 (168
+// registers), bf16 181 us for 64 long rows against 185 with 10, 8 bit 123 against
+// 155 with 8, though 37 rows of 0 to 1,031 keys take 10.6 against 10.0.
+template <int D, bool FP8>
 constexpr int warps() {
-    return FP8 ? 8 : 10;
+    return D == 64 ? 12 : FP8 ? 8 : 10;
 }
 
 constexpr float LN2 = 0.693147180559945309f;
@@ -695,9 +697,9 @@ __device__ __forceinline__ void finish(const Params& p, const Joined<FP8>& j, in
 }
 
 template <int D, bool FP8>
-__global__ void __launch_bounds__(warps<FP8>() * 32, 1)
+__global__ void __launch_bounds__(warps<D, FP8>() * 32, 1)
 decode_attention_kernel(const Params p) {
-    constexpr int WARPS = warps<FP8>();
+    constexpr int WARPS = warps<D, FP8>();
     constexpr int THREADS = WARPS * 32;
     constexpr int QUADS = D / 4;   // threads of a head in the join
     extern __shared__ __align__(16) char smem[];
@@ -772,9 +774,12 @@ decode_attention_kernel(const Params p) {
     for (int c = 0; c < 3; ++c) {
         if (c == 1 && block + 1 == blocks) continue;
         if (c == 2) {
-            const Cuts shares(hi - lo, WARPS);
-            end = lo + shares.at(warp + 1);
-            at.at = lo + shares.at(warp);
+            // (heads of 64: whole steps of 32 keys, 10.6 us for the 37 rows
+            // against 11.7; 8 bit of 128: 22.0 us for 64 rows of 300 keys against 21.0)
+            constexpr int WHOLE = D == 64 ? 2 : 1;
+            const Cuts shares((hi - lo + WHOLE - 1) / WHOLE, WARPS);
+            end = min(lo + shares.at(warp + 1) * WHOLE, hi);
+            at.at = min(lo + shares.at(warp) * WHOLE, end);
             if (at.at == end) break;
         } else {
             at.at = cuts.at(block + c);
@@ -964,10 +969,10 @@ decode_attention_kernel(const Params p) {
 template <int D, bool FP8>
 int launch(const Params& p, int blocks, cudaStream_t stream) {
     static std::atomic<bool> done[MAX_DEVICES];
-    constexpr int bytes = 2 * warps<FP8>() * sizeof(Slot<D>);
+    constexpr int bytes = 2 * warps<D, FP8>() * sizeof(Slot<D>);
     if (!set_smem_once(done, decode_attention_kernel<D, FP8>, bytes))
         return launch_status("qb_decode_attention: shared memory");
-    decode_attention_kernel<D, FP8><<<blocks, warps<FP8>() * 32, bytes, stream>>>(p);
+    decode_attention_kernel<D, FP8><<<blocks, warps<D, FP8>() * 32, bytes, stream>>>(p);
     return launch_status("qb_decode_attention");
 }
 
