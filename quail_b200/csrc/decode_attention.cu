@@ -34,12 +34,14 @@
 // one row and one tile of 8 query heads, its units are steps of 16 keys, and
 // the items' units laid end to end are cut into equal ranges, one for each
 // resident block, and a block's range into one for each warp. One line holds all
-// heads, item after item; for heads of 64 there is a line for each tile of
-// heads, cut alike, where the SMs divide so (8 KV heads: 18 blocks each, 4 of 148
-// left over): blocks next to each other then walk the same keys of neighbouring
-// heads, whose short rows lie together in memory (64 rows of 4k to 16k keys, 8
-// KV heads: 181 us against 207, 8 bit 123 against 164; heads of 128, 8 bit: 217
-// both ways, bf16 690 us against 696). A warp walks
+// heads, item after item; where a head's rows are short (heads of 64, or 8 bit)
+// there is a line for each tile of heads, cut alike, if the SMs divide so (8 KV
+// heads: 18 blocks each, 4 of 148 left over): blocks next to each other then walk
+// the same keys of neighbouring heads, whose rows lie together in memory. 8 KV
+// heads of 64, 64 rows of 4k to 16k keys: 181 us against 207, 8 bit 123 against
+// 164. 8-bit heads of 128: 256 rows of 96 to 2,112 keys 87.6 us against 96.6, one
+// of 40,960 27.2 against 29.4, 64 long ones 217 both ways, 16 long ones 59.6
+// against 58.6. bf16 of 128, one line: 128 long rows 673 us against 684. A warp walks
 // its range alone; items that lie within it are finished there, the parts of
 // the others (two a warp at most) meet in shared memory at the block's end,
 // and parts of an item that blocks share in the workspace: the block that
@@ -94,7 +96,7 @@ struct Params {
     int unit_shift;                   // log2 of the keys of a unit of work
     int n_q, n_kv, group;             // group = n_q / n_kv
     int tiles;                        // ceil(group / HEADS) items share a KV head
-    int lines;                        // lines of units (D = 64): n_kv * tiles, or 1
+    int lines;                        // lines of units (not bf16 of 128): n_kv * tiles, or 1
     const void* k;
     const void* v;
     const uint8_t* k_scale;
@@ -709,7 +711,7 @@ decode_attention_kernel(const Params p) {
     __shared__ uint32_t s_joins[2];
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     // block `block` of the line's `width` ones
-    const int lines = D == 64 ? p.lines : 1;
+    const int lines = D == 64 || FP8 ? p.lines : 1;
     const int line = blockIdx.x % lines, block = blockIdx.x / lines;
     const int width = gridDim.x / lines;
     const int per_row = p.n_kv * p.tiles / lines;   // items of a row in a line
