@@ -22,12 +22,11 @@
 // against 693.)
 //
 // Measured on a B200 (copy rate 6.55 TB/s), 32 query heads over 8 KV heads of
-// 128: 128 rows of 8,192 keys 642 us, 6.69 TB/s (8 bit: 402 us, 5.39 TB/s);
+// 128: 128 rows of 8,192 keys 643 us, 6.68 TB/s (8 bit: 340 us, 6.38 TB/s);
 // 256 rows of 96 to 2,112 keys 118 us, 88% of the copy rate; one row of 40,960
 // keys 37 us, 70%, a quarter of it the start and the join; one row of 37 keys
-// 5.3 us. The 8-bit cache is slower by the byte: its 128-byte rows, 1 KB apart,
-// reach 81% where one KV head's rows lie together at 89%, and a step's 574
-// instructions a warp leave two warps a scheduler little to hide latency with.
+// 5.3 us. 8 bit, 16 rows of 4k to 16k keys under 64 query heads: 55 us, 73%, some
+// 10 us of it the start and the join.
 //
 // Split and join. The rows' lengths are known on the device only (a captured
 // launch serves every step), so the blocks share the work there: an item is
@@ -39,9 +38,9 @@
 // heads: 18 blocks each, 4 of 148 left over): blocks next to each other then walk
 // the same keys of neighbouring heads, whose rows lie together in memory. 8 KV
 // heads of 64, 64 rows of 4k to 16k keys: 181 us against 207, 8 bit 123 against
-// 164. 8-bit heads of 128: 256 rows of 96 to 2,112 keys 87.6 us against 96.6, one
-// of 40,960 27.2 against 29.4, 64 long ones 217 both ways, 16 long ones 59.6
-// against 58.6. bf16 of 128, one line: 128 long rows 673 us against 684. A warp walks
+// 164. 8-bit heads of 128, with prefetches(): 64 long rows 188 us against 214, 256 of
+// 96 to 2,112 keys 83.5 against 97.8, one of 40,960 24.7 against 27.7, 37 of 1 to
+// 1,031 17.0 against 16.1. bf16 of 128, one line: 128 long rows 673 us against 684. A warp walks
 // its range alone; items that lie within it are finished there, the parts of
 // the others (two a warp at most) meet in shared memory at the block's end,
 // and parts of an item that blocks share in the workspace: the block that
@@ -69,7 +68,7 @@ constexpr int WHOLE_UNITS = 16, SHORT_UNITS = 28;
 // next step's K and V beside this one's. bf16: 10 (168 registers) 674 us for 128
 // rows of 4k to 16k keys, 116 for 256 rows of 96 to 2,112, 37.6 for one of 40,960;
 // 8 692, 122 and 38.0; 12 666, 118 and 39.5; 16 spills (867). 8 bit: 8 (255
-// registers) 60 us for 16 long rows, 10 spills (72). Heads of 64: 12 (168
+// registers), before the prefetch 60 us for 16 long rows, 10 spills (72). Heads of 64: 12 (168
 // registers), bf16 181 us for 64 long rows against 185 with 10, 8 bit 123 against
 // 155 with 8, though 37 rows of 0 to 1,031 keys take 10.6 against 10.0.
 template <int D, bool FP8>
@@ -233,6 +232,18 @@ __device__ __forceinline__ float e8m0_float(uint32_t b) {
     return __uint_as_float(b ? b << 23 : 0x00400000u);
 }
 
+// Whether a step's rows are prefetched to L2, one step before they are loaded. Where
+// heads have lines of their own, the lines walk the same keys in step, so each
+// prefetches the rows of all heads for its share of a step's keys: memory is
+// read 1 KB at a time in place of 128 bytes (8 KV heads, 64 rows of 4k to 16k
+// keys 188 us against 217, 81% -> 94% of the copy rate; each line's own rows
+// prefetched: 214). Further ahead is no better (190 us two steps, 197 four). Heads
+// of 64 lose (139 us against 123).
+template <int D, bool FP8>
+constexpr bool prefetches() {
+    return FP8 && D == 128;
+}
+
 // A warp's part of an item in shared memory (the padding keeps the rows of
 // neighbouring heads on different banks).
 template <int D>
@@ -248,12 +259,15 @@ static_assert(sizeof(Slot<64>) % 16 == 0 && sizeof(Slot<128>) % 16 == 0,
               "the slots' outputs are read as float4");
 
 // One warp: keys [key0, end) of row `row`, KV head kvh, query heads head0 ..
-// head0 + heads - 1; the result to `slot`.
+// head0 + heads - 1; the result to `slot`. prefetched: the key of a step (<< 16)
+// and the head whose K and V this lane prefetches (AHEAD).
 //
 // Lanes: g = lane / 4, t = lane % 4, as the MMA fragments number them.
 template <int D, bool FP8>
 __device__ __forceinline__ void attend(const Params& p, Slot<D>& slot, int row, int kvh,
-                                       int head0, int heads, int key0, int end, int lane) {
+                                       int head0, int heads, int key0, int end, int lane,
+                                       uint32_t prefetched) {
+    constexpr bool AHEAD = prefetches<D, FP8>();
     constexpr int ELEM = FP8 ? 1 : 2;
     constexpr int KC = D * ELEM / 64;            // 16-byte chunks of a K row a lane
     constexpr int VC = FP8 ? 1 : D / 64;         // chunks of a V row a lane
@@ -329,8 +343,8 @@ __device__ __forceinline__ void attend(const Params& p, Slot<D>& slot, int row, 
 #pragma unroll
         for (int j = 0; j < 4; ++j) o[i][j] = 0.0f;
 
-    // A step: 16 keys of 128 bf16, else 32 (8 bit, D = 128: 59.4 us for 16 long
-    // rows against 61.5 with 16 keys and 12 warps). The pipeline: while a step is
+    // A step: 16 keys of 128 bf16, else 32 (8 bit, D = 128, before the
+    // prefetch: 59.4 us for 16 long rows against 61.5 with 16 keys and 12 warps). The pipeline: while a step is
     // computed, the next one's K (as soon as S has consumed the registers), V
     // (after the second product) and, one further, the page ids are on their
     // way. Keys past the end are taken as the last one, with a weight of zero.
@@ -412,11 +426,30 @@ __device__ __forceinline__ void attend(const Params& p, Slot<D>& slot, int row, 
         }
     };
 
+    // The page of the lane's prefetched key, and the prefetch, a step later
+    uint32_t page = 0;
+    auto find_ahead = [&](int from) {
+        const int key = min(from + (int)(prefetched >> 16), end - 1);
+        if (AHEAD) page = (uint32_t)__ldg(table + (key >> p.page_shift));
+    };
+    auto prefetch = [&](int from) {
+        const int key = from + (int)(prefetched >> 16);
+        if (!AHEAD || key >= end || page >= n_pages) return;
+        const uint64_t at =
+            (uint64_t)((page << p.page_shift) + ((uint32_t)key & mask)) * row_bytes +
+            (prefetched & 0xFFFFu) * (D * ELEM);
+        asm volatile("prefetch.global.L2 [%0];" ::"l"((const char*)p.k + at));
+        asm volatile("prefetch.global.L2 [%0];" ::"l"((const char*)p.v + at));
+    };
+
     find(key0);
+    find_ahead(key0 + STEP);
     load_k(key0);
+    prefetch(key0 + STEP);
     load_v();
     lost = next_lost;
     find(key0 + STEP);
+    find_ahead(key0 + 2 * STEP);
     for (; key0 < end; key0 += STEP) {
         // the scales of keys g and g + 8: a factor, and (values) an exponent,
         // the byte as a float by way of a mantissa
@@ -463,6 +496,8 @@ __device__ __forceinline__ void attend(const Params& p, Slot<D>& slot, int row, 
         // (past the end: the last key again; behind a branch these loads are not
         // moved up: 740 us against 670 for 128 long rows)
         load_k(key0 + STEP);
+        prefetch(key0 + 2 * STEP);
+        find_ahead(key0 + 3 * STEP);
         // x, and y = x and the value's exponent: [2 * half + head]
         float x[UNITS][4], y[UNITS][4];
 #pragma unroll
@@ -715,6 +750,12 @@ decode_attention_kernel(const Params p) {
     const int line = blockIdx.x % lines, block = blockIdx.x / lines;
     const int width = gridDim.x / lines;
     const int per_row = p.n_kv * p.tiles / lines;   // items of a row in a line
+    // piece kvh * 32 + lane of a step's 32 keys by all KV heads (prefetches())
+    uint32_t prefetched = 0;
+    if (prefetches<D, FP8>() && lines > 1) {
+        const uint32_t piece = (uint32_t)(line / p.tiles * 32 + lane);
+        prefetched = piece / (uint32_t)p.n_kv << 16 | piece % (uint32_t)p.n_kv;
+    }
 
     // ---- a scan over the rows' units: up to 32 rows by every warp for itself, a
     // row a lane (one short row 5.3 us against 5.9); more by the block, `chunk`
@@ -825,10 +866,12 @@ decode_attention_kernel(const Params p) {
             const int kvh = item / p.tiles, tile = item % p.tiles;
             const int head0 = kvh * p.group + tile * HEADS;
             const int heads = min(HEADS, p.group - tile * HEADS);
+            if (lines == 1) prefetched = (uint32_t)lane << 16 | (uint32_t)kvh;
             const int whole = 2 * (at.at == s) + (stop == s + n);
             Slot<D>& slot = slots[2 * warp + (at.at == s)];
             attend<D, FP8>(p, slot, at.row, kvh, head0, heads, (at.at - s) << p.unit_shift,
-                           (int)min((int64_t)keys, (int64_t)(stop - s) << p.unit_shift), lane);
+                           (int)min((int64_t)keys, (int64_t)(stop - s) << p.unit_shift), lane,
+                           prefetched);
             __syncwarp();
             if (whole == 3) {
                 for (int i = lane; i < HEADS * QUADS; i += 32) {
