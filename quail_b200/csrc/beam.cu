@@ -12,11 +12,12 @@
 // an addition in fp32. A block keeps its n_out best so far as sorted keys
 // (value, lower token first), and a bar: first the n_out-th largest of the
 // first tile's 32 groups' maxima, later the last of the best. Logits that
-// pass are put on a list, without a barrier, and the list is ranked after 9,
-// 81, ... tiles and at the end: of a run in no order about 8 n_out pass between. Where more pass than the list
-// holds (logits that rise along the run, or many equal ones), the run is gone
-// through again tile by tile, each thread that has a logit which passes
-// putting its best forward, and again, until none does. The block that completes its group (a counter) joins the runs and the beams, in an
+// pass are put on a list, without a barrier, and the list is ranked after 9, 81,
+// ... tiles and at the end: of a run in no order about 8 n_out pass between.
+// Where more pass than the list holds (logits that rise along the run, or many
+// equal ones), the run is gone through again tile by tile, each thread that has a
+// logit which passes putting its best forward, and again, until none does. The
+// block that completes its group (a counter) joins the runs and the beams, in an
 // order that does not depend on who came last.
 //
 // Measured on a B200, vocabulary 151,936: 16 groups of 8 beams, bf16 19 us (31%

@@ -38,15 +38,17 @@
 // heads: 18 blocks each, 4 of 148 left over): blocks next to each other then walk
 // the same keys of neighbouring heads, whose rows lie together in memory. 8 KV
 // heads of 64, 64 rows of 4k to 16k keys: 181 us against 207, 8 bit 123 against
-// 164. 8-bit heads of 128, with prefetches(): 64 long rows 188 us against 214, 256 of
-// 96 to 2,112 keys 83.5 against 97.8, one of 40,960 24.7 against 27.7, 37 of 1 to
-// 1,031 17.0 against 16.1. bf16 of 128, one line: 128 long rows 673 us against 684. A warp walks
-// its range alone; items that lie within it are finished there, the parts of
-// the others (two a warp at most) meet in shared memory at the block's end,
-// and parts of an item that blocks share in the workspace: the block that
-// completes the item (a counter per cut) joins its parts in the blocks' order,
-// so the result does not depend on who came last. Nothing waits. A block's cut
-// that would part a short item, or leave a sliver, moves to the item's edge.
+// 164. 8-bit heads of 128, with prefetches(): 64 long rows 188 us against 214, 256
+// of 96 to 2,112 keys 83.5 against 97.8, one of 40,960 24.7 against 27.7, 37 of 1
+// to 1,031 17.0 against 16.1. bf16 of 128 in one line: 128 long rows 673 us against
+// 684. (With lines and prefetches() both 663, but 256 ragged rows 121 against 118
+// and 37 rows 15.0 against 13.8.) A warp walks its range alone; items that lie
+// within it are finished there, the parts of the others (two a warp at most) meet
+// in shared memory at the block's end, and parts of an item that blocks share in
+// the workspace: the block that completes the item (a counter per cut) joins its
+// parts in the blocks' order, so the result does not depend on who came last.
+// Nothing waits. A block's cut that would part a short item, or leave a sliver,
+// moves to the item's edge.
 #include <cuda_fp16.h>
 
 #include "common.cuh"
@@ -68,9 +70,9 @@ constexpr int WHOLE_UNITS = 16, SHORT_UNITS = 28;
 // next step's K and V beside this one's. bf16: 10 (168 registers) 674 us for 128
 // rows of 4k to 16k keys, 116 for 256 rows of 96 to 2,112, 37.6 for one of 40,960;
 // 8 692, 122 and 38.0; 12 666, 118 and 39.5; 16 spills (867). 8 bit: 8 (255
-// registers), before the prefetch 60 us for 16 long rows, 10 spills (72). Heads of 64: 12 (168
-// registers), bf16 181 us for 64 long rows against 185 with 10, 8 bit 123 against
-// 155 with 8, though 37 rows of 0 to 1,031 keys take 10.6 against 10.0.
+// registers), 60 us for 16 long rows before the prefetch, 10 spills (72). Heads of
+// 64: 12 (168 registers), bf16 181 us for 64 long rows against 185 with 10, 8 bit
+// 123 against 155 with 8, though 37 rows of 0 to 1,031 keys take 10.6 against 10.0.
 template <int D, bool FP8>
 constexpr int warps() {
     return D == 64 ? 12 : FP8 ? 8 : 10;
@@ -343,11 +345,12 @@ __device__ __forceinline__ void attend(const Params& p, Slot<D>& slot, int row, 
 #pragma unroll
         for (int j = 0; j < 4; ++j) o[i][j] = 0.0f;
 
-    // A step: 16 keys of 128 bf16, else 32 (8 bit, D = 128, before the
-    // prefetch: 59.4 us for 16 long rows against 61.5 with 16 keys and 12 warps). The pipeline: while a step is
-    // computed, the next one's K (as soon as S has consumed the registers), V
-    // (after the second product) and, one further, the page ids are on their
-    // way. Keys past the end are taken as the last one, with a weight of zero.
+    // A step: 16 keys of 128 bf16, else 32 (8 bit, D = 128, before the prefetch:
+    // 59.4 us for 16 long rows against 61.5 with 16 keys and 12 warps). The
+    // pipeline: while a step is computed, the next one's K (as soon as S has
+    // consumed the registers), V (after the second product) and, one further, the
+    // page ids are on their way. Keys past the end are taken as the last one, with
+    // a weight of zero.
     constexpr int UNITS = FP8 || D == 64 ? 2 : 1;
     constexpr int STEP = 16 * UNITS;
     const uint32_t row_bytes = (uint32_t)p.n_kv * (D * ELEM);
@@ -703,7 +706,8 @@ __device__ __forceinline__ void finish(const Params& p, const Joined<FP8>& j, in
     }
     if (live) {
         if (p.lse && d4 == 0)
-            p.lse[row * (int64_t)p.n_q + head] = j.l != 0.0f ? (j.m + log2_approx(j.l)) * LN2 : NEG_INF;
+            p.lse[row * (int64_t)p.n_q + head] =
+                j.l != 0.0f ? (j.m + log2_approx(j.l)) * LN2 : NEG_INF;
         if (p.out) {
             uint2 b;
             b.x = bf16x2_bits(r[0], r[1]);

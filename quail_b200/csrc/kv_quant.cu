@@ -269,7 +269,8 @@ extern "C" int qb_kv_quant_write(const void* k, const void* v, int64_t k_ld, int
     auto* kernel = head_dim == 128 ? kv_quant_write_kernel<128> : kv_quant_write_kernel<64>;
     kernel<<<blocks, THREADS, 0, (cudaStream_t)stream>>>(
         (const bf16*)k, (const bf16*)v, k_ld, v_ld, src, dst, n, src_rows, n_kv,
-        chunks, per_block, (uint8_t*)k_codes, (uint8_t*)v_codes, k_scale, v_scale, pool_rows, status);
+        chunks, per_block, (uint8_t*)k_codes, (uint8_t*)v_codes, k_scale, v_scale, pool_rows,
+        status);
     return launch_status(who);
 }
 
