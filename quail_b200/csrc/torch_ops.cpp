@@ -3,7 +3,7 @@
 //
 // A decode step makes several small calls a layer, each a few microseconds on
 // the GPU; through ctypes and Python-level checks one costs 12 to 16 us of host
-// time, here 6 to 8. The library's entry points are bound by address (bind), so
+// time, here 4 to 7. The library's entry points are bound by address (bind), so
 // this module follows whichever libquailb200 is loaded.
 #include <c10/core/DeviceGuard.h>
 #include <c10/cuda/CUDAGraphsC10Utils.h>
