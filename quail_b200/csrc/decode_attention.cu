@@ -509,12 +509,14 @@ __device__ __forceinline__ void attend(const Params& p, Slot<D>& slot, int row, 
             for (int h = 0; h < 2; ++h) {
                 const bool in =
                     key0 + 16 * u + 8 * h + g < end && !(now_lost >> (2 * u + h) & 1);
+                // (a key that is left out has pool row 0's exponent, perhaps a NaN)
+                const float plus = FP8 && in ? more[u][h] : 0.0f;
 #pragma unroll
                 for (int n = 0; n < 2; ++n) {
                     const float z =
                         s[u][2 * h + n] * (FP8 ? by[u][h] * x_scale[n] : x_scale[n]);
                     x[u][2 * h + n] = in ? z : NEG_INF;
-                    y[u][2 * h + n] = FP8 ? x[u][2 * h + n] + more[u][h] : 0.0f;
+                    y[u][2 * h + n] = FP8 ? x[u][2 * h + n] + plus : 0.0f;
                 }
             }
         float most[2], most_v[2];
