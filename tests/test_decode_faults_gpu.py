@@ -1,5 +1,11 @@
-"""Decode attention on the GPU where keys are left out, against the formulas in
-64 bits (the bounds are those of tests/test_decode_gpu.py).
+"""Decode attention on the GPU where keys are left out or nearly cancel, against
+the formulas in 64 bits (the bounds are those of tests/test_decode_gpu.py).
+
+Where V's contributions cancel, the output is small beside sum w |v|, so its
+rounding to bf16 hides nothing of the weights' own: a weight is off by
+expm1(2 dx) against the normaliser, 2^-20 for the exponential and its rounding
+for the second product, 2^-16 for a pair of bf16 or of f16 numbers (22 bits of
+the latter, of which subnormals may drop some).
 """
 
 import math
@@ -52,3 +58,34 @@ def test_keys_of_bad_pages_are_left_out(dev, quant, n_q, n_kv, d):  # noqa: F811
     left.lengths = [len(r) for r in rows]
     assert left.lengths[3] == 0
     left.check(out, lse)
+
+
+@pytest.mark.parametrize("d", [64, 128])
+@pytest.mark.parametrize("quant", [False, True])
+def test_values_that_cancel(dev, quant, d):  # noqa: F811
+    """Half of the keys weigh 1 and hold the value 1, the others weigh about 2/3
+    and hold -3/2: the output is what the weights' rounding leaves."""
+    n = 32
+    case = Case(dev, 8, 1, d, [n], quant=quant, seed=3, spare=0)
+    case.q[:] = 0
+    case.q[:, :, 0] = 1.0
+    odd = (torch.arange(n, device=dev) % 2).view(n, 1, 1)
+    k = torch.zeros(n, 1, d, dtype=torch.bfloat16, device=dev)
+    k[:, :, :1] = -odd.to(torch.bfloat16)
+    v = torch.where(odd == 1, -1.5, 1.0).to(torch.bfloat16).expand(n, 1, d).contiguous()
+    at = case.rows_of(0)
+    if quant:
+        decode.kv_quant_write(k, v, case.kv, at)
+    else:
+        case.kv[0][at], case.kv[1][at] = k, v
+    for step in range(24):
+        scale = math.log(1.5) + (step - 12) * 2.0 ** -11
+        out = decode.decode_attention(case.q, case.kv, case.table, case.used,
+                                      softmax_scale=scale)
+        b = math.exp(-scale)
+        want, size = (1 - 1.5 * b) / (1 + b), (1 + 1.5 * b) / (1 + b)
+        dx = d / 16 * 2 ** -20.8 * scale
+        dw = math.expm1(2 * dx) + 2 ** -16 + 2 ** -20 + (n / 16 + 32) * 2 ** -21
+        bound = dw * size + 2 ** -8 * (1 + dw) * abs(want)
+        assert float((out.double() - want).abs().max()) <= bound, (step, want, out[0, 0, :2])
+    assert status() == 0
