@@ -162,8 +162,9 @@ class Generator:
         return eng.final_norm(hidden, residual, every, w.final_norm)
 
     def logits(self, normed):
-        """The tied output head over the whole vocabulary (bf16)."""
-        return normed @ self.weights.embed.t()
+        """The tied output head over the whole vocabulary, f32: in bf16 logits of
+        16 and more are steps of 1/8 apart, and so would the scores be."""
+        return self.torch.mm(normed, self.weights.embed.t(), out_dtype=self.torch.float32)
 
     def generate(self, prompts, max_new_tokens, beams=1, eos=None):
         """Completion per prompt (token ids, at least one each): up to
