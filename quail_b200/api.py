@@ -103,7 +103,6 @@ class B200Executor:
         self.budget = cfg.max_chunk_tokens
         # pinned host / device input buffers reused by every chunk upload
         self.staging = InputStaging(torch, self.device)
-        self._generators = {}   # kv format -> Generator
 
     def reset_arena(self):
         """Free every page (the pools stay allocated)."""
@@ -213,7 +212,5 @@ class B200Executor:
         "fp8" over an 8-bit copy of the prompts' KV. Returns a
         generate.Completion (tokens and log-probability of each beam) per
         prompt; the arena's pages are free again afterwards."""
-        held = self._generators.get(kv)
-        if held is None:
-            held = self._generators[kv] = Generator(self, kv)
-        return held.generate(prompts, max_new_tokens, beams=beams, eos=eos)
+        # (one that is kept would keep this executor's memory in a cycle)
+        return Generator(self, kv).generate(prompts, max_new_tokens, beams=beams, eos=eos)
