@@ -209,7 +209,9 @@ class B200Executor:
     def generate(self, prompts, max_new_tokens, *, beams=1, eos=None, kv="bf16"):
         """Continue each prompt (token ids) by up to max_new_tokens tokens: beam
         search, greedy with one beam. kv: "bf16" decodes over the arena's pools,
-        "fp8" over an 8-bit copy of the prompts' KV. Returns a
+        "fp8" over an 8-bit cache in the arena's memory, at half the pages (beside
+        those of the longest prompt) and, for the call, 1 / head_dim of the
+        arena's bytes for scales. Returns a
         generate.Completion (tokens and log-probability of each beam) per
         prompt; the arena's pages are free again afterwards."""
         # (one that is kept would keep this executor's memory in a cycle)

@@ -48,6 +48,22 @@ class QuantKV:
                                  device=device)
         self.scales = torch.empty((n_layers, 2, rows, n_kv), dtype=torch.uint8, device=device)
 
+    @classmethod
+    def over(cls, arena):
+        """An 8-bit cache whose codes lie in an arena's own memory: the arena's page
+        p is the 8-bit pages 2p and 2p + 1, for whoever has reserved it. Only the
+        scale bytes are allocated, 1 / d_head of the arena's bytes."""
+        kv = cls.__new__(cls)
+        kv.n_layers, kv.n_pages, kv.page_tokens = (arena.n_layers, 2 * arena.n_pages,
+                                                   arena.page_tokens)
+        kv.n_kv, kv.d_head = arena.n_kv, arena.d_head
+        rows = kv.n_pages * kv.page_tokens
+        kv.codes = arena.pools.view(torch.float8_e4m3fn).view(kv.n_layers, 2, rows, kv.n_kv,
+                                                              kv.d_head)
+        kv.scales = torch.empty((kv.n_layers, 2, rows, kv.n_kv), dtype=torch.uint8,
+                                device=arena.pools.device)
+        return kv
+
     def layer_kv(self, layer: int) -> QuantLayer:
         return QuantLayer(self.codes[layer, 0], self.codes[layer, 1], self.scales[layer, 0],
                           self.scales[layer, 1])

@@ -9,7 +9,7 @@ prefill's own pipeline and arena:
     choose      the output head (tied embeddings), beam_select, beam_reorder
     step        embed + norm + quant, qkv GEMM + q/k norm + rotary, the new
                 token's KV written (bf16 into the arena, or 8-bit into a
-                QuantKV over the same pages), decode_attention quantised for
+                QuantKV over its memory), decode_attention quantised for
                 o_proj, the MLP, the final norm
 
 A row's beams share the full pages of its prompt (the arena's borrowing) and
@@ -43,9 +43,11 @@ class Generator:
     Args:
         executor: api.B200Executor; its arena must have pages free for the
             rows generated at once.
-        kv: "bf16" decodes over the arena's pools; "fp8" quantises the prompts'
-            KV into an 8-bit cache over the same page ids after the prefill and
-            decodes over that, at half the bytes a step.
+        kv: "bf16" decodes over the arena's pools; "fp8" over an 8-bit cache in
+            pages of the arena's memory, at half the bytes a token and a step.
+            The prompts then pass through bf16 pages, a prefill chunk at a time;
+            where a few rows' cache and the longest prompt do not fit together,
+            the cache gets memory of its own for the call.
     """
 
     def __init__(self, executor, kv="bf16"):
@@ -56,35 +58,67 @@ class Generator:
         self.pipeline = executor.pipeline
         self.arena = executor.arena
         self.weights = executor.weights
-        self.quant = None
-        if kv == "fp8":
-            a = self.arena
-            self.quant = decode.QuantKV(a.n_layers, a.n_pages, a.page_tokens, a.n_kv, a.d_head,
-                                        device=executor.device)
+        self.kv = kv
+        self.quant = None   # the 8-bit cache of a call
         self.workspace = decode.decode_workspace(executor.device)
 
     # ---- pages ------------------------------------------------------------------
 
     def _reserve(self, prompts, new_tokens, beams):
-        """Arena keys of every beam, row by row: beam 0 holds the prompt, the
-        others borrow its full pages; each owns pages for its own tokens."""
-        arena, keys = self.arena, []
+        """The arena keys that hold the rows' pages. bf16: one a beam, row by row:
+        beam 0 holds the prompt, the others borrow its full pages; each owns pages
+        for its own tokens. 8-bit: one for all of them, or none."""
+        arena, keys, self.quant = self.arena, [], None
+        pages = sum(sum(self._beam_pages(p, new_tokens, beams)) for p in prompts)
+        # two 8-bit pages lie in one of the arena's, beside the longest prompt's
+        # bf16 ones; or those alone are the arena's
+        half, longest = -(-pages // 2), arena.pages_needed(max(len(p) for p in prompts))
+        inside = self.kv == "fp8" and half + longest <= arena.free_pages
+        if not inside and pages > arena.free_pages:
+            raise RuntimeError(
+                f"the arena is short of pages for {len(prompts)} rows of {beams} beams and "
+                f"{new_tokens} tokens (free: {arena.free_pages})")
+
+        def hold(key, tokens, **kw):
+            arena.alloc(key, tokens, **kw)
+            keys.append(key)
         try:
-            for i, prompt in enumerate(prompts):
-                n, full = len(prompt), len(prompt) // arena.page_tokens * arena.page_tokens
-                for b in range(beams):
-                    key = ("generate", (i, b))
-                    borrow = (("generate", (i, 0)), full) if b and full else None
-                    if arena.alloc(key, n, capacity_tokens=n + new_tokens,
-                                   borrow=borrow) is None:
-                        raise RuntimeError(
-                            f"the arena is short of pages for {len(prompts)} rows of {beams} "
-                            f"beams and {new_tokens} tokens (free: {arena.free_pages})")
-                    keys.append(key)
+            if inside:
+                self.quant = decode.QuantKV.over(arena)
+                hold(("generate", "8-bit"), half * arena.page_tokens)
+            elif self.kv == "fp8":
+                self.quant = decode.QuantKV(arena.n_layers, pages, arena.page_tokens, arena.n_kv,
+                                            arena.d_head, device=arena.pools.device)
+            else:
+                for i, prompt in enumerate(prompts):
+                    n, full = len(prompt), len(prompt) // arena.page_tokens * arena.page_tokens
+                    for b in range(beams):
+                        borrow = (("generate", (i, 0)), full) if b and full else None
+                        hold(("generate", (i, b)), n, capacity_tokens=n + new_tokens,
+                             borrow=borrow)
         except Exception:
             self._release(keys)
             raise
         return keys
+
+    def _beam_pages(self, prompt, new_tokens, beams):
+        """(the pages that a row's beams share, those they own together)."""
+        full = len(prompt) // self.arena.page_tokens
+        return full, beams * (self.arena.pages_needed(len(prompt) + new_tokens) - full)
+
+    def _tables(self, prompts, new_tokens, beams, keys):
+        """The page ids of every beam, row by row."""
+        if self.quant is None:
+            return [self.arena.owned_pages(key) for key in keys]
+        ids = iter(range(self.quant.n_pages))
+        if keys:
+            ids = iter([2 * p + half for p in self.arena.owned_pages(keys[0]) for half in (0, 1)])
+        tables = []
+        for prompt in prompts:
+            shared, own = self._beam_pages(prompt, new_tokens, beams)
+            full = [next(ids) for _ in range(shared)]
+            tables += [full + [next(ids) for _ in range(own // beams)] for _ in range(beams)]
+        return tables
 
     def _release(self, keys):
         for key in reversed(keys):   # borrowers before the key they borrow from
@@ -92,33 +126,65 @@ class Generator:
 
     # ---- the passes ----------------------------------------------------------------
 
-    def _prefill(self, prompts, keys):
-        """Normed last rows [prompts, hidden]; every prompt token's KV written."""
-        torch, arena = self.torch, self.arena
-        normed, groups, tokens = [], [], 0
+    def _chunks(self, prompts):
+        """(first, end) of the prompts that one forward pass takes: up to the
+        executor's budget and, where they only pass through the arena, its free
+        pages."""
+        room = None if self.quant is None else self.arena.free_pages
+        first = tokens = pages = 0
+        for i, prompt in enumerate(prompts):
+            more = self.arena.pages_needed(len(prompt))
+            if i > first and (tokens + len(prompt) > self.executor.budget
+                              or (room is not None and pages + more > room)):
+                yield first, i
+                first, tokens, pages = i, 0, 0
+            tokens += len(prompt)
+            pages += more
+        yield first, len(prompts)
 
-        def flush():
-            chunk = pack_chunk(arena, groups, attention_mode="tree")
-            assert isinstance(chunk, HostChunk)
-            normed.append(self.pipeline.forward_chunk(
-                chunk.upload(torch, self.executor.device)))
+    def _prefill(self, prompts, keys=None, tables=None):
+        """Normed last rows [prompts, hidden]; every prompt token's KV written, to
+        the pages of its key (bf16) or of its table (8-bit)."""
+        normed = []
+        for first, end in self._chunks(prompts):
+            chunk = prompts[first:end]
+            if self.quant is None:
+                normed.append(self._forward(chunk, keys[first:end]))
+                continue
+            held = []
+            try:
+                for i, prompt in enumerate(chunk):
+                    self.arena.alloc(("generate", i), len(prompt))
+                    held.append(("generate", i))
+                normed.append(self._forward(chunk, held))
+                self._quantise(chunk, held, tables[first:end])
+            finally:
+                # (used again in stream order)
+                self._release(held)
+        return self.torch.cat(normed)
+
+    def _forward(self, prompts, keys):
+        groups = []
         for key, prompt in zip(keys, prompts):
-            if groups and tokens + len(prompt) > self.executor.budget:
-                flush()
-                groups, tokens = [], 0
             ids = np.asarray(prompt, dtype=np.int64)
             groups.append(dict(key=key, prefix=ids[:-1], f=len(ids) - 1, suffixes=[ids[-1:]],
                                write_suffix_tokens=1))
-            tokens += len(prompt)
-        flush()
-        if self.quant is not None:
-            rows = np.concatenate([arena.capacity_rows(key)[:len(p)]
-                                   for key, p in zip(keys, prompts)])
-            rows = torch.from_numpy(rows).to(self.executor.device)
-            for layer in range(arena.n_layers):
-                k, v = arena.layer_kv(layer)
-                decode.kv_quant_write(k, v, self.quant.layer_kv(layer), rows, src=rows)
-        return torch.cat(normed)
+        chunk = pack_chunk(self.arena, groups, attention_mode="tree")
+        assert isinstance(chunk, HostChunk)
+        return self.pipeline.forward_chunk(chunk.upload(self.torch, self.executor.device))
+
+    def _quantise(self, prompts, keys, tables):
+        """The prompts' KV from their keys' bf16 rows to the 8-bit rows of their
+        tables."""
+        arena, torch = self.arena, self.torch
+        page = np.arange(arena.page_tokens)
+        src = np.concatenate([arena.capacity_rows(key)[:len(p)] for key, p in zip(keys, prompts)])
+        dst = np.concatenate([(np.asarray(t)[:, None] * arena.page_tokens + page).reshape(-1)
+                              [:len(p)] for t, p in zip(tables, prompts)])
+        src, dst = (torch.from_numpy(x).to(self.executor.device) for x in (src, dst))
+        for layer in range(arena.n_layers):
+            k, v = arena.layer_kv(layer)
+            decode.kv_quant_write(k, v, self.quant.layer_kv(layer), dst, src=src)
 
     def step(self, tokens, positions, rows, table, used):
         """One token of every beam: normed rows [beams, hidden].
@@ -187,16 +253,17 @@ class Generator:
                 return self._search(prompts, keys, max_new_tokens, beams, eos)
         finally:
             self._release(keys)
+            self.quant = None
 
     def _search(self, prompts, keys, max_new_tokens, beams, eos):
         torch, dev, arena = self.torch, self.executor.device, self.arena
         groups, pad = len(prompts), 0 if eos is None else eos
-        pages = [arena.owned_pages(key) for key in keys]
+        pages = self._tables(prompts, max_new_tokens, beams, keys)
         table = torch.from_numpy(arena.block_table_rows(pages)).to(dev)
         used = torch.tensor([len(p) for p in prompts], dtype=torch.int32, device=dev)
         pools = (arena.pools,) if self.quant is None else self.quant.pools
 
-        normed = self._prefill(prompts, keys[::beams])
+        normed = self._prefill(prompts, keys[::beams], pages[::beams])
         # every beam's first token comes from the prompt's own row
         scores, parents, tokens = decode.beam_select(
             self.logits(normed), torch.zeros(groups, 1, device=dev), n_out=beams)
