@@ -213,6 +213,7 @@ class B200Executor:
         those of the longest prompt) and, for the call, 1 / head_dim of the
         arena's bytes for scales. Returns a
         generate.Completion (tokens and log-probability of each beam) per
-        prompt; the arena's pages are free again afterwards."""
+        prompt; the arena's pages are free again afterwards. Where the arena is
+        short of pages, retained keys are evicted."""
         # (one that is kept would keep this executor's memory in a cycle)
         return Generator(self, kv).generate(prompts, max_new_tokens, beams=beams, eos=eos)

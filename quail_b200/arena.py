@@ -434,6 +434,14 @@ class KVArena:
             self.evict_key(victim[0])
         return tuple(evicted)
 
+    def evictable_pages(self) -> int:
+        """Pages that would come free if every retained key were evicted (those
+        held for queued borrowers stay)."""
+        acct = self.accounting
+        gone = {key for key in acct.retained if key not in self._holds}
+        kept = {page for key in acct.owned if key not in gone for page in acct.table_pages(key)}
+        return len({page for key in gone for page in acct.table_pages(key)} - kept)
+
     def evict_key(self, key) -> int:
         """Free one retained key and count the KV lost."""
         tokens = self.accounting.tokens[key]

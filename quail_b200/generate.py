@@ -41,8 +41,9 @@ class Generator:
     """Beam search (greedy with one beam) on one executor's model.
 
     Args:
-        executor: api.B200Executor; its arena must have pages free for the
-            rows generated at once.
+        executor: api.B200Executor; its arena must have pages for the rows
+            generated at once, free or held by retained keys, which are evicted
+            in their order as far as needed.
         kv: "bf16" decodes over the arena's pools; "fp8" over an 8-bit cache in
             pages of the arena's memory, at half the bytes a token and a step.
             The prompts then pass through bf16 pages, a prefill chunk at a time;
@@ -73,11 +74,20 @@ class Generator:
         # two 8-bit pages lie in one of the arena's, beside the longest prompt's
         # bf16 ones; or those alone are the arena's
         half, longest = -(-pages // 2), arena.pages_needed(max(len(p) for p in prompts))
-        inside = self.kv == "fp8" and half + longest <= arena.free_pages
-        if not inside and pages > arena.free_pages:
+        ways = [(pages, longest if self.kv == "fp8" else pages, False)]
+        if self.kv == "fp8":
+            ways.insert(0, (half + longest, half + longest, True))
+        room = arena.free_pages
+        fit = next((w for w in ways if w[0] <= room), None)
+        if fit is None:   # with what is kept for later operators
+            room += arena.evictable_pages()
+            fit = next((w for w in ways if w[0] <= room), None)
+        if fit is None:
             raise RuntimeError(
                 f"the arena is short of pages for {len(prompts)} rows of {beams} beams and "
                 f"{new_tokens} tokens (free: {arena.free_pages})")
+        _, need, inside = fit
+        arena.evict_retained(need - arena.free_pages)
 
         def hold(key, tokens, **kw):
             arena.alloc(key, tokens, **kw)

@@ -98,3 +98,57 @@ def test_an_executor_ends_with_its_last_reference(kv):
         assert gone() is None
     finally:
         gc.enable()
+
+
+def retained(ex, n, tokens, alias="doc"):
+    for i in range(n):
+        assert ex.arena.alloc((alias, i), tokens) is not None
+        ex.arena.retain((alias, i), tokens)
+
+
+@pytest.mark.parametrize("kv", ["bf16", "fp8"])
+def test_retained_keys_give_way(kv):
+    """Keys kept for a later operator are evicted, as few as needed, where the
+    arena is short; pinned ones are not."""
+    ex = B200Executor(torch, CFG, 60, seed=3)
+    rows = prompts(5, [64, 64])           # 6 pages each in bf16
+    want = ex.generate(rows, 20, kv=kv)
+    retained(ex, 15, 62)                  # 4 pages each: the arena is full
+    assert ex.arena.free_pages == 0
+    got = ex.generate(rows, 20, kv=kv)
+    assert [o.tokens for o in got] == [o.tokens for o in want]
+    # bf16: 12 pages; 8 bit: 6, and 4 for a prompt on its way through
+    assert len(ex.arena.retained_keys()) == 12 and ex.arena.free_pages == 12
+    for key in ex.arena.retained_keys():
+        ex.arena.pin(key)
+    held = ex.arena.free_pages
+    with pytest.raises(RuntimeError, match="short of pages"):
+        ex.generate(rows * 4, 20, kv=kv)
+    assert ex.arena.free_pages == held
+    ex.arena.reset()
+
+
+def test_nothing_is_evicted_for_rows_that_never_fit():
+    ex = B200Executor(torch, CFG, 60, seed=3)
+    retained(ex, 5, 62)
+    for key in [("doc", 0), ("doc", 1)]:
+        ex.arena.pin(key)
+    with pytest.raises(RuntimeError, match="short of pages"):
+        ex.generate(prompts(6, [64] * 9), 20)        # 54 pages of at most 52
+    assert len(ex.arena.retained_keys()) == 3
+    ex.arena.reset()
+
+
+def test_generation_after_a_filter_that_retains():
+    """Through the executor's own calls: a filter keeps its survivors' KV in a
+    nearly full arena, generation takes their pages."""
+    ex = B200Executor(torch, CFG, 48, seed=3)
+    docs = prompts(7, [60] * 10)          # 4 pages each
+    result = ex.filter(docs, [[7]], keys=[("t", i) for i in range(10)], retain_survivors=True,
+                       budget=128)
+    kept = len(ex.arena.retained_keys())
+    assert kept == int(result.bits.sum()) and ex.arena.free_pages == 48 - 4 * kept
+    out = ex.generate(prompts(8, [64] * 7), 20)      # 42 pages
+    assert len(out) == 7
+    assert len(ex.arena.retained_keys()) <= 1
+    ex.arena.reset()
