@@ -66,9 +66,18 @@ def _compile(src: Path, verbose_ptxas: bool) -> Path:
     return obj
 
 
+def _torch_build() -> str:
+    """The torch and Python that _torch_ops.so is compiled for."""
+    import torch
+    return (f"torch {torch.__version__}, C++11 ABI {int(torch._C._GLIBCXX_USE_CXX11_ABI)}, "
+            f"{sysconfig.get_config_var('SOABI')}")
+
+
 def _build_torch_ops(force: bool) -> Path:
     src = CSRC / "torch_ops.cpp"
-    if not force and not _stale(TORCH_OPS, [src, *INCLUDE.glob("*.h")]):
+    built_for, now = BUILD_DIR / "torch_ops.for", _torch_build()
+    same = built_for.exists() and built_for.read_text() == now
+    if not force and same and not _stale(TORCH_OPS, [src, *INCLUDE.glob("*.h")]):
         return TORCH_OPS
     import torch
     root = Path(torch.__file__).parent
@@ -84,6 +93,7 @@ def _build_torch_ops(force: bool) -> Path:
     if proc.returncode != 0:
         raise RuntimeError(f"g++ failed on {src.name}:\n{proc.stdout}\n{proc.stderr}")
     os.replace(tmp, TORCH_OPS)
+    built_for.write_text(now)
     return TORCH_OPS
 
 
