@@ -24,7 +24,7 @@
 // of the copy rate), f32 24 us (49%); 4 beams of one group 8.4 us. Of the 19 us,
 // the exponentials alone need 4.4 (16 a clock an SM) and reading 6; a block's
 // start, its ranking and the join of the group take the latency of about ten
-// dependent steps.
+// dependent steps. (64 registers a thread, for 1,024 an SM; 36 bytes are spilled.)
 #include "common.cuh"
 
 namespace {

@@ -22,10 +22,10 @@
 // against 693.)
 //
 // Measured on a B200 (copy rate 6.55 TB/s), 32 query heads over 8 KV heads of
-// 128: 128 rows of 8,192 keys 643 us, 6.68 TB/s (8 bit: 340 us, 6.38 TB/s);
-// 256 rows of 96 to 2,112 keys 118 us, 88% of the copy rate; one row of 40,960
+// 128: 128 rows of 8,192 keys 643 us, 6.68 TB/s (8 bit: 341 us, 6.35 TB/s);
+// 256 rows of 96 to 2,112 keys 119 us, 87% of the copy rate; one row of 40,960
 // keys 37 us, 70%, a quarter of it the start and the join; one row of 37 keys
-// 5.3 us. 8 bit, 16 rows of 4k to 16k keys under 64 query heads: 55 us, 73%, some
+// 5.3 us. 8 bit, 16 rows of 4k to 16k keys under 64 query heads: 56 us, 72%, some
 // 10 us of it the start and the join.
 //
 // Split and join. The rows' lengths are known on the device only (a captured
@@ -37,10 +37,10 @@
 // there is a line for each tile of heads, cut alike, if the SMs divide so (8 KV
 // heads: 18 blocks each, 4 of 148 left over): blocks next to each other then walk
 // the same keys of neighbouring heads, whose rows lie together in memory. 8 KV
-// heads of 64, 64 rows of 4k to 16k keys: 181 us against 207, 8 bit 123 against
-// 164. 8-bit heads of 128, with prefetches(): 64 long rows 188 us against 214, 256
-// of 96 to 2,112 keys 83.5 against 97.8, one of 40,960 24.7 against 27.7, 37 of 1
-// to 1,031 17.0 against 16.1. bf16 of 128 in one line: 128 long rows 673 us against
+// heads of 64, 64 rows of 4k to 16k keys: 180 us against 206, 8 bit 126 against
+// 164. 8-bit heads of 128, with prefetches(): 64 long rows 189 us against 217, 256
+// of 96 to 2,112 keys 86 against 99, one of 40,960 25.2 against 29.9, 37 of 1
+// to 1,031 17.4 against 16.4. bf16 of 128 in one line: 128 long rows 673 us against
 // 684. (With lines and prefetches() both 663, but 256 ragged rows 121 against 118
 // and 37 rows 15.0 against 13.8.) A warp walks its range alone; items that lie
 // within it are finished there, the parts of the others (two a warp at most) meet
@@ -67,12 +67,14 @@ constexpr int MIN_UNITS = 8;    // a block's least part of an item that is cut
 constexpr int WHOLE_UNITS = 16, SHORT_UNITS = 28;
 
 // Warps of a block, one block an SM: as many as leave the registers for the
-// next step's K and V beside this one's. bf16: 10 (168 registers) 674 us for 128
-// rows of 4k to 16k keys, 116 for 256 rows of 96 to 2,112, 37.6 for one of 40,960;
-// 8 692, 122 and 38.0; 12 666, 118 and 39.5; 16 spills (867). 8 bit: 8 (255
-// registers), 60 us for 16 long rows before the prefetch, 10 spills (72). Heads of
-// 64: 12 (168 registers), bf16 181 us for 64 long rows against 185 with 10, 8 bit
-// 123 against 155 with 8, though 37 rows of 0 to 1,031 keys take 10.6 against 10.0.
+// next step's K and V beside this one's, give or take a few bytes. bf16: 10 (168
+// registers; 20 bytes spilled and 28 filled a thread) 689 us for 128 rows of 4k to
+// 16k keys, 119 for 256 rows of 96 to 2,112, 36.6 for one of 40,960; 8 (no spill)
+// 704, 122 and 37.0; 12 680, 119 and 38.0; 16 spills much (867). 8 bit: 8 (254
+// registers), 189 us for 64 long rows, 10 spills (258). Heads of 64: 12 (168
+// registers; bf16 16 bytes spilled, 24 filled), bf16 180 us for 64 long rows against
+// 184 with 10, 8 bit 126 against 157 with 8, though 37 rows of 0 to 1,031 keys take
+// 11.0 against 10.1.
 template <int D, bool FP8>
 constexpr int warps() {
     return D == 64 ? 12 : FP8 ? 8 : 10;
@@ -242,9 +244,9 @@ __device__ __forceinline__ float e8m0_float(uint32_t b) {
 // heads have lines of their own, the lines walk the same keys in step, so each
 // prefetches the rows of all heads for its share of a step's keys: memory is
 // read 1 KB at a time in place of 128 bytes (8 KV heads, 64 rows of 4k to 16k
-// keys 188 us against 217, 81% -> 94% of the copy rate; each line's own rows
-// prefetched: 214). Further ahead is no better (190 us two steps, 197 four). Heads
-// of 64 lose (139 us against 123).
+// keys 189 us against 216, 81% -> 93% of the copy rate; each line's own rows
+// prefetched: 192). Two steps ahead are no better (189 us; one row of 40,960 keys
+// 26.3 against 25.2). Heads of 64 lose (139 us against 126).
 template <int D, bool FP8>
 constexpr bool prefetches() {
     return FP8 && D == 128;
@@ -836,8 +838,8 @@ decode_attention_kernel(const Params p) {
     for (int c = 0; c < 3; ++c) {
         if (c == 1 && block + 1 == blocks) continue;
         if (c == 2) {
-            // (heads of 64: whole steps of 32 keys, 10.6 us for the 37 rows
-            // against 11.7; 8 bit of 128: 22.0 us for 64 rows of 300 keys against 21.0)
+            // (heads of 64: whole steps of 32 keys, 11.0 us for the 37 rows
+            // against 12.1; 8 bit of 128: 22.0 us for 64 rows of 300 keys against 21.2)
             constexpr int WHOLE = D == 64 ? 2 : 1;
             const Cuts shares((hi - lo + WHOLE - 1) / WHOLE, WARPS);
             end = min(lo + shares.at(warp + 1) * WHOLE, hi);
