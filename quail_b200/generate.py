@@ -71,8 +71,10 @@ class Generator:
         for its own tokens. 8-bit: one for all of them, or none."""
         arena, keys, self.quant = self.arena, [], None
         pages = sum(sum(self._beam_pages(p, new_tokens, beams)) for p in prompts)
-        # two 8-bit pages lie in one of the arena's, beside the longest prompt's
-        # bf16 ones; or those alone are the arena's
+        # The arena's pages that a way of placing them asks for, and takes, and
+        # whether an 8-bit cache lies inside: two of its pages in one of the arena's,
+        # beside the longest prompt's bf16 ones. Else those alone are the arena's, and
+        # the cache lies beside it where the arena could hold the rows in bf16.
         half, longest = -(-pages // 2), arena.pages_needed(max(len(p) for p in prompts))
         ways = [(pages, longest if self.kv == "fp8" else pages, False)]
         if self.kv == "fp8":
